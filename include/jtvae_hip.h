@@ -37,7 +37,7 @@
 extern "C" {
 #endif
 
-#define JTVAE_ABI_VERSION 19
+#define JTVAE_ABI_VERSION 20
 
 #define JTVAE_E_NULL (-1)     /* required pointer is NULL            */
 #define JTVAE_E_SHAPE (-2)    /* negative / inconsistent sizes       */
@@ -508,6 +508,117 @@ int jtvae_row_dot_bwd(const float* dscore, const float* q, const int32_t* owner,
  * (jtprop_vae.py:454-473). */
 int jtvae_segment_ce(const float* scores, const int32_t* seg_ptr, const int32_t* label_pos, int32_t n_seg,
                      float* loss_seg, int32_t* hit_seg, float* dscores, void* stream);
+
+/* ---- log-probabilities of labels under rows of logits, and the losses built on them ----------
+ * No counterpart in the reference (its only losses are the teacher-forced ones of fast_jtnn/jtnn_dec.py and
+ * jtnn_vae.py): what fine-tuning the decoder on preferred molecules or on a reward needs. */
+
+/* element types of logits, parameters and gradients */
+#define JTVAE_F32 0
+#define JTVAE_F16 1
+#define JTVAE_BF16 2
+
+typedef struct jtvae_logits {
+  const void* x;       /* [n_rows, ld], row i = logits of position i; natural alignment only            */
+  int32_t dtype;       /* JTVAE_F32 / F16 / BF16                                                        */
+  int64_t ld;          /* elements from row to row, >= n_cols                                           */
+  int32_t n_rows, n_cols;
+  const void* labels;  /* [n_rows] int32 or int64; < 0: the row has no label and is not read            */
+  int32_t label_bits;  /* 32 or 64                                                                      */
+} jtvae_logits_t;
+
+/* stats[i] = (max_j x_ij, sum_j exp(x_ij - max)); log_probs[i] = log softmax(x_i)[label_i] as fp32 and / or fp64
+ * (either may be NULL), 0 without a label.  owner (or NULL): rows with owner[i] < 0 count as rows without a label.
+ * A label >= n_cols gives NaN, as does a row whose logits are all -inf or hold NaN or +inf. */
+int jtvae_label_log_probs(const jtvae_logits_t* logits, const int32_t* owner, float* stats, float* log_probs,
+                          double* log_probs64, void* stream);
+
+/* dx[i, j] = c_i ([j = label_i] - softmax(x_i)_j) in the logits' type, c_i = coef[owner ? owner[i] : i] * upstream
+ * (device scalar, or NULL = 1); rows without a label get zeros.  Columns [n_cols, width) are padding and
+ * become zero (n_cols <= width <= ld_dx). */
+int jtvae_label_log_probs_bwd(const jtvae_logits_t* logits, const int32_t* owner, const float* stats,
+                              const float* coef, const float* upstream, void* dx, int64_t ld_dx, int64_t width,
+                              void* stream);
+
+/* sums[q] = sum of log_probs64 over rows[rowptr[q] .. rowptr[q+1]) (+ other[q]); sums64: the same unrounded, or
+ * NULL.  Fixed order: bitwise reproducible. */
+int jtvae_sequence_sums(const double* log_probs64, const int32_t* rowptr, const int32_t* rows, int32_t n_seq,
+                        const float* other, double* sums64, float* sums, void* stream);
+
+/* pairs[p] = (preferred, other) sequence.  margin_p = beta ((sums64 - ref)[preferred] - (sums64 - ref)[other]);
+ * loss = scale * sum_p -(1 - smoothing) log sigmoid(margin_p) - smoothing log sigmoid(-margin_p);
+ * coef[q] = d loss / d sums64[q].  seq_ptr / seq_pairs: CSR of the pairs that name sequence q, as 2 p + side.
+ * dmargin: scratch [n_pairs]. */
+int jtvae_preference_pairs(const double* sums64, const float* ref, const int32_t* pairs, int32_t n_pairs,
+                           const int32_t* seq_ptr, const int32_t* seq_pairs, int32_t n_seq, double beta,
+                           double smoothing, double scale, float* loss, float* margins, double* dmargin, float* coef,
+                           void* stream);
+
+typedef struct jtvae_policy {
+  const float* old_log_probs; /* [n_rows] log-probability of the label when it was sampled             */
+  const float* advantages;    /* [n_rows]                                                              */
+  const float* ref_log_probs; /* [n_rows] under the reference model, or NULL: no KL term               */
+  const float* weights;       /* [n_rows], or NULL = 1                                                 */
+  double clip_low, clip_high; /* the ratio is clipped to [1 - clip_low, 1 + clip_high]                 */
+  double kl_coef, scale;
+} jtvae_policy_t;
+
+/* r = exp(lp - old), k3 = exp(ref - lp) - (ref - lp) - 1, w = scale * weights:
+ * *loss = sum w (kl_coef k3 - min(r A, clip(r) A)) over the rows with a label, *kl = sum w k3, *clipped = sum of w over
+ * the rows whose ratio was clipped (device scalars); coef[i] = d loss / d lp_i; log_probs and stats as above. */
+size_t jtvae_policy_loss_workspace_bytes(int32_t n_rows);
+int jtvae_policy_loss(const jtvae_logits_t* logits, const jtvae_policy_t* policy, float* stats, float* log_probs,
+                      float* coef, float* loss, float* kl, float* clipped, void* workspace, size_t workspace_bytes,
+                      void* stream);
+
+/* ---- AdamW over many tensors ----------------------------------------------------------------- */
+
+#define JTVAE_ADAMW_BLOCK 256        /* elements of a tensor that share one scale of the 8-bit states       */
+#define JTVAE_ADAMW_CHUNK 4096       /* elements of a tensor one workgroup updates                          */
+#define JTVAE_ADAMW_MAX_TENSORS 400  /* gradient addresses one launch carries; longer lists take several    */
+
+/* One parameter tensor, contiguous; this table is DEVICE memory.  States start at 16-byte boundaries. */
+typedef struct jtvae_adamw_tensor {
+  void* param;         /* dtype of the group                                                        */
+  float* master;       /* fp32 copy the step works on (16-bit parameters), or NULL                  */
+  void* exp_avg;       /* fp32, or e4m3 values                                                      */
+  void* second;        /* fp32 exp_avg_sq, or e4m3 values of its square root                        */
+  float* exp_avg_scale;/* 8-bit states: one scale per JTVAE_ADAMW_BLOCK elements; else NULL         */
+  float* second_scale;
+  int64_t n;
+} jtvae_adamw_tensor_t;
+
+typedef struct jtvae_adamw_group {
+  const jtvae_adamw_tensor_t* tensors; /* device [n_tensors]                                           */
+  const int32_t* chunks;       /* device [n_chunks, 2]: tensor and chunk inside the tensor, tensor by tensor */
+  const int64_t* chunk_ptr;    /* HOST [n_tensors + 1]: first chunk of every tensor                    */
+  const void* const* grads;    /* HOST [n_tensors]: gradient of every tensor, same type, contiguous; NULL = skip it */
+  int32_t* steps;              /* device [n_tensors]: steps every tensor has made                      */
+  float* bias;                 /* device [n_tensors, 2]: scratch, the bias corrections of this step    */
+  int32_t n_tensors;
+  int64_t n_chunks;
+  int32_t dtype;               /* JTVAE_F32 / F16 / BF16                                               */
+  int32_t state_bits;          /* 32 or 8                                                              */
+  int32_t use_master;          /* 16-bit parameters: the step works on the tensors' master copies      */
+  const float* lr_device;      /* device scalar that replaces lr, or NULL                              */
+  double lr, beta1, beta2, eps, weight_decay;
+} jtvae_adamw_group_t;
+
+/* partials[c] = sum of squares of the gradient elements of chunk c (0 where there is no gradient), [n_chunks]. */
+int jtvae_grad_square_sums(const jtvae_adamw_group_t* group, double* partials, void* stream);
+
+/* norm[0] = sqrt(sum of partials), norm[1] = min(1, max_norm / (norm[0] + 1e-6)): what every gradient is multiplied by
+ * to bring their common 2-norm down to max_norm. */
+int jtvae_grad_norm(const double* partials, int64_t n_partials, double max_norm, float* norm, void* stream);
+
+/* One step of the tensors that have a gradient.  g = grad * *grad_scale (device scalar, or NULL = 1), t = ++steps:
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
+ *   w = w (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * on the fp32 copy where there is one, whose rounded value then becomes the parameter.  8-bit states hold m and
+ * sqrt(v) as e4m3 values times the block's scale max / 448, rounded to nearest after the update; a root that is not
+ * zero keeps at least the smallest value 2^-9, so that it never leaves m divided by eps alone.  A maximum of at most
+ * 2^-100 counts as zero.  An element that is not finite becomes NaN and leaves the rest of its block as it is. */
+int jtvae_adamw_step(const jtvae_adamw_group_t* group, const float* grad_scale, void* stream);
 
 /* ---- host-side index preparation (host memory in and out; no GPU work, no stream) ---------- */
 

@@ -10,8 +10,11 @@ from .jtmpn import JTMPN
 from .jtnn_dec import JTNNDecoder
 from .jtnn_enc import GraphGRU, JTNNEncoder
 from .jtnn_vae import JTNNVAE, JTpropVAE
+from .losses import SequencePlan, policy_loss, preference_loss, sequence_log_probs, token_log_probs
 from .mpn import MPN
 from .nnutils import create_var, gather_sum, index_select_ND
+from .optim import AdamW
 
 __all__ = ["MPN", "JTNNEncoder", "GraphGRU", "JTMPN", "JTNNDecoder", "JTNNVAE", "JTpropVAE", "create_var",
-           "gather_sum", "index_select_ND"]
+           "gather_sum", "index_select_ND", "SequencePlan", "token_log_probs", "sequence_log_probs", "preference_loss",
+           "policy_loss", "AdamW"]

@@ -26,7 +26,9 @@ LIB_PATH = os.environ.get("JTVAE_HIP_LIB") or os.path.join(_HERE, "libjtvae_hip.
 
 ACT_NONE, ACT_RELU, ACT_SIGMOID, ACT_TANH = 0, 1, 2, 3
 EPI_PLAIN, EPI_GRU_BLEND, EPI_MUL_ACC = 0, 1, 2
-ABI_VERSION = 19
+ABI_VERSION = 20
+F32, F16, BF16 = 0, 1, 2
+DTYPE_CODE = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 
 
 class Epilogue(C.Structure):
@@ -180,9 +182,32 @@ class TreeCsrC(C.Structure):
                  ("max_sf", C.c_int32)])
 
 
+class Logits(C.Structure):  # jtvae_logits_t
+    _fields_ = [("x", C.c_void_p), ("dtype", C.c_int32), ("ld", C.c_int64), ("n_rows", C.c_int32),
+                ("n_cols", C.c_int32), ("labels", C.c_void_p), ("label_bits", C.c_int32)]
+
+
+class Policy(C.Structure):  # jtvae_policy_t
+    _fields_ = ([(n, C.c_void_p) for n in ("old_log_probs", "advantages", "ref_log_probs", "weights")] +
+                [(n, C.c_double) for n in ("clip_low", "clip_high", "kl_coef", "scale")])
+
+
+class AdamwTensor(C.Structure):  # jtvae_adamw_tensor_t
+    _fields_ = ([(n, C.c_void_p) for n in ("param", "master", "exp_avg", "second", "exp_avg_scale", "second_scale")] +
+                [("n", C.c_int64)])
+
+
+class AdamwGroup(C.Structure):  # jtvae_adamw_group_t
+    _fields_ = ([(n, C.c_void_p) for n in ("tensors", "chunks", "chunk_ptr", "grads", "steps", "bias")] +
+                [("n_tensors", C.c_int32), ("n_chunks", C.c_int64), ("dtype", C.c_int32), ("state_bits", C.c_int32),
+                 ("use_master", C.c_int32), ("lr_device", C.c_void_p)] +
+                [(n, C.c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay")])
+
+
+ADAMW_BLOCK, ADAMW_CHUNK = 256, 4096
 PACK_MAX = 16
 E_NULL, E_SHAPE, E_ALIGN, E_RANGE, E_WORKSPACE = -1, -2, -3, -4, -5
-_i32, _vp, _sz, _i64 = C.c_int32, C.c_void_p, C.c_size_t, C.c_int64
+_i32, _vp, _sz, _i64, _f64 = C.c_int32, C.c_void_p, C.c_size_t, C.c_int64, C.c_double
 
 # name -> (restype, argtypes); must list every function of include/jtvae_hip.h
 SIGNATURES = {
@@ -237,6 +262,16 @@ SIGNATURES = {
     "jtvae_onehot_linear": (C.c_int, [_vp, _i32, _i32, _vp, _i32, _vp, _vp, _i32, _i32, _vp]),
     "jtvae_onehot_linear_bwd_workspace_bytes": (_sz, [_i32, _i32, _i32]),
     "jtvae_onehot_linear_bwd": (C.c_int, [_vp, _i32, _i32, _vp, _i32, _i32, _vp, _i32, _i32, _vp, _sz, _vp]),
+    "jtvae_label_log_probs": (C.c_int, [C.POINTER(Logits), _vp, _vp, _vp, _vp, _vp]),
+    "jtvae_label_log_probs_bwd": (C.c_int, [C.POINTER(Logits), _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp]),
+    "jtvae_sequence_sums": (C.c_int, [_vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp]),
+    "jtvae_preference_pairs": (C.c_int, [_vp, _vp, _vp, _i32, _vp, _vp, _i32, _f64, _f64, _f64, _vp, _vp, _vp, _vp,
+                                         _vp]),
+    "jtvae_policy_loss_workspace_bytes": (_sz, [_i32]),
+    "jtvae_policy_loss": (C.c_int, [C.POINTER(Logits), C.POINTER(Policy), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "jtvae_grad_square_sums": (C.c_int, [C.POINTER(AdamwGroup), _vp, _vp]),
+    "jtvae_grad_norm": (C.c_int, [_vp, _i64, _f64, _vp, _vp]),
+    "jtvae_adamw_step": (C.c_int, [C.POINTER(AdamwGroup), _vp, _vp]),
     "jtvae_tensorize_graph_counts": (C.c_int, [_vp, _vp, _i64, _vp, _vp]),
     "jtvae_tensorize_graphs": (C.c_int, [_vp, _vp, _i64, _i32, _vp, _vp, _vp, _i32]),
     "jtvae_tensorize_tree_counts": (C.c_int, [_vp, _vp, _i64, _i32, _i32, _vp]),
@@ -650,6 +685,61 @@ def row_dot(score, q, owner, cand, n_cand, H, ld, n_owner=None):
 def row_dot_bwd(dscore, q, owner, cand, own_ptr, n_cand, n_owner, dq, dcand, H, ld):
     _run("row_dot_bwd", lib.jtvae_row_dot_bwd, (dscore, q, owner, cand, own_ptr, n_cand, n_owner, dq, dcand, H, ld,
                                                 stream_ptr()), nbytes=4 * H * (2 * n_cand + 2 * n_owner) + 12 * n_cand)
+
+
+def logits_arg(x, ld, n_rows, n_cols, dtype, labels, label_bits):
+    return Logits(x, dtype, ld, n_rows, n_cols, labels, label_bits)
+
+
+def _logits_bytes(g):
+    return g.n_rows * g.n_cols * (4 if g.dtype == F32 else 2)
+
+
+def label_log_probs(g, owner, stats, log_probs, log_probs64):
+    _run("label_log_probs", lib.jtvae_label_log_probs,
+         (C.byref(g), owner, stats, log_probs, log_probs64, stream_ptr()), nbytes=_logits_bytes(g) + 24 * g.n_rows)
+
+
+def label_log_probs_bwd(g, owner, stats, coef, upstream, dx, ld_dx, width):
+    _run("label_log_probs_bwd", lib.jtvae_label_log_probs_bwd,
+         (C.byref(g), owner, stats, coef, upstream, dx, ld_dx, width, stream_ptr()), nbytes=2 * _logits_bytes(g) + 20 * g.n_rows)
+
+
+def sequence_sums(log_probs64, rowptr, rows, n_seq, other, sums64, sums, n_rows=0):
+    _run("sequence_sums", lib.jtvae_sequence_sums,
+         (log_probs64, rowptr, rows, n_seq, other, sums64, sums, stream_ptr()), nbytes=12 * n_rows + 20 * n_seq)
+
+
+def preference_pairs(sums64, ref, pairs, n_pairs, seq_ptr, seq_pairs, n_seq, beta, smoothing, scale, loss, margins,
+                     dmargin, coef):
+    _run("preference_pairs", lib.jtvae_preference_pairs,
+         (sums64, ref, pairs, n_pairs, seq_ptr, seq_pairs, n_seq, beta, smoothing, scale, loss, margins, dmargin, coef,
+          stream_ptr()), nbytes=40 * n_pairs + 20 * n_seq)
+
+
+def policy_loss_workspace_bytes(n_rows):
+    return int(lib.jtvae_policy_loss_workspace_bytes(n_rows))
+
+
+def policy_loss(g, policy, stats, log_probs, coef, loss, kl, clipped, ws, ws_bytes):
+    _run("policy_loss", lib.jtvae_policy_loss,
+         (C.byref(g), C.byref(policy), stats, log_probs, coef, loss, kl, clipped, ws, ws_bytes,
+          stream_ptr()), nbytes=_logits_bytes(g) + 40 * g.n_rows)
+
+
+def grad_square_sums(group, partials, n_elems=0):
+    _run("grad_square_sums", lib.jtvae_grad_square_sums, (C.byref(group), partials, stream_ptr()),
+         nbytes=n_elems * (4 if group.dtype == F32 else 2))
+
+
+def grad_norm(partials, n_partials, max_norm, norm):
+    _run("grad_norm", lib.jtvae_grad_norm, (partials, n_partials, max_norm, norm, stream_ptr()), nbytes=8 * n_partials)
+
+
+def adamw_step(group, grad_scale, n_elems=0):
+    size = 4 if group.dtype == F32 else 2
+    per = 3 * size + (16 if group.state_bits == 32 else 4) + (8 - size if group.use_master else 0)
+    _run("adamw_step", lib.jtvae_adamw_step, (C.byref(group), grad_scale, stream_ptr()), nbytes=n_elems * per)
 
 
 # ---- host-side index preparation (numpy arrays in host memory; no GPU involved) -----------------
