@@ -535,10 +535,11 @@ int jtvae_label_log_probs(const jtvae_logits_t* logits, const int32_t* owner, fl
 
 /* dx[i, j] = c_i ([j = label_i] - softmax(x_i)_j) in the logits' type, c_i = coef[owner ? owner[i] : i] * upstream
  * (device scalar, or NULL = 1); rows without a label get zeros.  Columns [n_cols, width) are padding and
- * become zero (n_cols <= width <= ld_dx). */
+ * become zero (n_cols <= width <= ld_dx).  unless_one: dx holds the gradient for upstream = 1 already, nothing is done
+ * if *upstream is 1. */
 int jtvae_label_log_probs_bwd(const jtvae_logits_t* logits, const int32_t* owner, const float* stats,
-                              const float* coef, const float* upstream, void* dx, int64_t ld_dx, int64_t width,
-                              void* stream);
+                              const float* coef, const float* upstream, int32_t unless_one, void* dx, int64_t ld_dx,
+                              int64_t width, void* stream);
 
 /* sums[q] = sum of log_probs64 over rows[rowptr[q] .. rowptr[q+1]) (+ other[q]); sums64: the same unrounded, or
  * NULL.  Fixed order: bitwise reproducible. */
@@ -565,11 +566,12 @@ typedef struct jtvae_policy {
 
 /* r = exp(lp - old), k3 = exp(ref - lp) - (ref - lp) - 1, w = scale * weights:
  * *loss = sum w (kl_coef k3 - min(r A, clip(r) A)) over the rows with a label, *kl = sum w k3, *clipped = sum of w over
- * the rows whose ratio was clipped (device scalars); coef[i] = d loss / d lp_i; log_probs and stats as above. */
+ * the rows whose ratio was clipped (device scalars); coef[i] = d loss / d lp_i; log_probs and stats as above.
+ * dx (or NULL): the gradient of loss with respect to the logits, as jtvae_label_log_probs_bwd gives it. */
 size_t jtvae_policy_loss_workspace_bytes(int32_t n_rows);
 int jtvae_policy_loss(const jtvae_logits_t* logits, const jtvae_policy_t* policy, float* stats, float* log_probs,
-                      float* coef, float* loss, float* kl, float* clipped, void* workspace, size_t workspace_bytes,
-                      void* stream);
+                      float* coef, float* loss, float* kl, float* clipped, void* dx, int64_t ld_dx, int64_t width,
+                      void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- AdamW over many tensors ----------------------------------------------------------------- */
 

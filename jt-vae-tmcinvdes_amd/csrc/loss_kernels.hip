@@ -63,68 +63,327 @@ __device__ __forceinline__ double label_log_prob(const T* row, long label, int n
   return ((double)(float)row[label] - (double)st.m) - log((double)st.s);
 }
 
-// One block per row.
+// Sixteen bytes of a row.  Rows start wherever the element type may stand (odd vocabularies, sliced views): the
+// hardware takes a 16-byte access at any address, and a wave's 1 KiB then touches nine cache lines instead of eight.
+typedef unsigned Word4 __attribute__((ext_vector_type(4)));
+typedef unsigned Word4At2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned Word4At4 __attribute__((ext_vector_type(4), aligned(4)));
+
 template <typename T>
-__global__ __launch_bounds__(JTVAE_BLOCK) void row_stats_kernel(const T* __restrict__ x, long ld, int n_cols,
-                                                                Labels labels, const int* __restrict__ owner,
-                                                                float2* __restrict__ stats, float* __restrict__ lp32,
-                                                                double* __restrict__ lp64) {
+struct Vec {
+  static constexpr int E = 16 / sizeof(T);
+  static __device__ __forceinline__ Word4 load(const T* p) { return *(const Word4At2*)p; }
+  static __device__ __forceinline__ void store(T* p, Word4 w) { *(Word4At2*)p = w; }
+  static __device__ __forceinline__ void unpack(Word4 w, float v[E]) {
+    T h[E];
+    __builtin_memcpy(h, &w, 16);
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = (float)h[e];
+  }
+  static __device__ __forceinline__ Word4 pack(const float v[E]) {
+    T h[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) h[e] = (T)v[e];
+    Word4 w;
+    __builtin_memcpy(&w, h, 16);
+    return w;
+  }
+};
+template <>
+struct Vec<float> {
+  static constexpr int E = 4;
+  static __device__ __forceinline__ Word4 load(const float* p) { return *(const Word4At4*)p; }
+  static __device__ __forceinline__ void store(float* p, Word4 w) { *(Word4At4*)p = w; }
+  static __device__ __forceinline__ void unpack(Word4 w, float v[4]) { __builtin_memcpy(v, &w, 16); }
+  static __device__ __forceinline__ Word4 pack(const float v[4]) {
+    Word4 w;
+    __builtin_memcpy(&w, v, 16);
+    return w;
+  }
+};
+
+// Takes the N values of v into st: their maximum first, then one exponential each.
+template <int N>
+__device__ __forceinline__ void take(RowStat& st, const float* v) {
+  float top = v[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) top = fmaxf(top, v[i]);
+  const float m = fmaxf(st.m, top), ref = finite_or_zero(m);
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) s += exp_nat(v[i] - ref);
+  st.s = st.s * exp_nat(st.m - ref) + s;
+  st.m = m;
+}
+
+// PolicyRow: r = exp(lp - old), term = w (kl_coef k3 - min(r A, clip(r) A)), k3 = exp(ref - lp) - (ref - lp) - 1
+// (an unbiased, never negative estimate of the KL divergence from the sampled label alone), and
+// d term / d lp = w (kl_coef (1 - exp(ref - lp)) - [r A <= clip(r) A] r A).
+struct PolicyRow {
+  double loss, kl, clipped;
+  float coef;
+};
+
+struct PolicyIn {
+  const float *old_lp, *adv, *ref, *weights;
+  double lo, hi, kl_coef, scale;
+};
+
+__device__ __forceinline__ PolicyRow policy_row(const PolicyIn& in, int row, double lp) {
+  PolicyRow o;
+  const double w = in.scale * (in.weights ? (double)in.weights[row] : 1.0);
+  const double a = (double)in.adv[row], r = exp(lp - (double)in.old_lp[row]);
+  const double plain = r * a, cut = (r < in.lo ? in.lo : (r > in.hi ? in.hi : r)) * a;
+  const bool clipped = cut < plain;
+  double k3 = 0.0, dk3 = 0.0;
+  if (in.ref) {
+    const double gap = (double)in.ref[row] - lp, e = expm1(gap);
+    k3 = e - gap;
+    dk3 = -e;
+  }
+  o.loss = w * (in.kl_coef * k3 - (clipped ? cut : plain));
+  o.kl = w * k3;
+  o.clipped = clipped ? w : 0.0;
+  o.coef = (float)(w * (in.kl_coef * dk3 - (clipped ? 0.0 : plain)));
+  return o;
+}
+
+template <typename T>
+struct RowsIn {
+  const T* x;
+  long ld;
+  int n_rows, n_cols;
+  Labels labels;
+  const int* owner;
+  float2* stats;
+  float* lp32;
+  double* lp64;
+};
+
+// What a row's end leaves behind: statistics and the log-probability in the types asked for.
+template <typename T>
+__device__ __forceinline__ double finish_row(const RowsIn<T>& in, int row, long label, bool counted, RowStat st) {
+  const double lp = counted ? label_log_prob(in.x + (long)row * in.ld, label, in.n_cols, st) : 0.0;
+  if (in.stats) in.stats[row] = counted ? make_float2(st.m, st.s) : make_float2(0.f, 1.f);
+  if (in.lp32) in.lp32[row] = (float)lp;
+  if (in.lp64) in.lp64[row] = lp;
+  return lp;
+}
+
+template <typename T>
+__device__ __forceinline__ bool counts(const RowsIn<T>& in, int row, long label) {
+  return label >= 0 && !(in.owner && in.owner[row] < 0);
+}
+
+// Statistics of one long row per block, streamed: four 16-byte loads in flight per lane.  Reads at the rate of the
+// memory; a row of any length.
+template <typename T, int BLOCK>
+__global__ __launch_bounds__(BLOCK) void stats_kernel(RowsIn<T> in) {
+  constexpr int E = Vec<T>::E, U = 4;
+  __shared__ RowStat part[BLOCK / 64];
   const int row = blockIdx.x;
-  const long label = labels[row];
-  __shared__ RowStat part[JTVAE_BLOCK / 64];
-  if (label < 0 || (owner && owner[row] < 0)) {
-    if (threadIdx.x == 0) {
-      stats[row] = make_float2(0.f, 1.f);
-      if (lp32) lp32[row] = 0.f;
-      if (lp64) lp64[row] = 0.0;
-    }
+  const long label = in.labels[row];
+  if (!counts(in, row, label)) {
+    if (threadIdx.x == 0) finish_row(in, row, label, false, RowStat{0.f, 1.f});
     return;
   }
-  const T* r = x + (long)row * ld;
+  const T* r = in.x + (long)row * in.ld;
+  const int n_vec = in.n_cols / E;
   RowStat st = {-INFINITY, 0.f};
-  for (int c = threadIdx.x; c < n_cols; c += JTVAE_BLOCK) {
-    const float v = (float)r[c], m = fmaxf(st.m, v), ref = finite_or_zero(m);
-    st.s = st.s * exp_nat(st.m - ref) + exp_nat(v - ref);
-    st.m = m;
+  int i = threadIdx.x;
+  for (; i + (U - 1) * BLOCK < n_vec; i += U * BLOCK) {
+    Word4 w[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) w[u] = Vec<T>::load(r + (long)(i + u * BLOCK) * E);
+    float v[U * E];
+#pragma unroll
+    for (int u = 0; u < U; ++u) Vec<T>::unpack(w[u], v + u * E);
+    take<U * E>(st, v);
+  }
+  for (; i < n_vec; i += BLOCK) {
+    float v[E];
+    Vec<T>::unpack(Vec<T>::load(r + (long)i * E), v);
+    take<E>(st, v);
+  }
+  const int c = n_vec * E + threadIdx.x;
+  if (c < in.n_cols) {
+    const float v = (float)r[c];
+    take<1>(st, &v);
   }
   st = wave_join(st);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = st;
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int w = 1; w < JTVAE_BLOCK / 64; ++w) st = join(st, part[w]);
-    stats[row] = make_float2(st.m, st.s);
-    const double lp = label_log_prob(r, label, n_cols, st);
-    if (lp32) lp32[row] = (float)lp;
-    if (lp64) lp64[row] = lp;
+    for (int w = 1; w < BLOCK / 64; ++w) st = join(st, part[w]);
+    finish_row(in, row, label, true, st);
   }
 }
 
-// dx[row, j] = c ([j = label] - exp(x_j - m) / s), c = coef[owner or row] * upstream.
 template <typename T>
-__global__ __launch_bounds__(JTVAE_BLOCK) void row_grad_kernel(const T* __restrict__ x, long ld, int n_cols,
-                                                               Labels labels, const int* __restrict__ owner,
-                                                               const float2* __restrict__ stats,
-                                                               const float* __restrict__ coef,
-                                                               const float* __restrict__ upstream,
-                                                               T* __restrict__ dx, long ld_dx, long width) {
-  const int row = blockIdx.x;
-  const long label = labels[row];
-  const int own = owner ? owner[row] : row;
-  T* d = dx + (long)row * ld_dx;
-  for (long c = n_cols + threadIdx.x; c < width; c += JTVAE_BLOCK) d[c] = (T)0.f;
-  if (label < 0 || own < 0) {
-    for (int c = threadIdx.x; c < n_cols; c += JTVAE_BLOCK) d[c] = (T)0.f;
-    return;
+struct GradOut {
+  T* dx;
+  long ld, width;
+};
+
+// -ks exp(x - m), plus k at the label.
+template <int E>
+__device__ __forceinline__ void softmax_grad(float v[E], long col, long label, float m, float ks, float k) {
+#pragma unroll
+  for (int e = 0; e < E; ++e) v[e] = -ks * exp_nat(v[e] - m);
+  const unsigned long at = (unsigned long)(label - col);
+  if (at < (unsigned long)E) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] += e == (int)at ? k : 0.f;
   }
-  const T* r = x + (long)row * ld;
-  float k = coef[own];
-  if (upstream) k *= *upstream;
-  if (label >= n_cols) k = NAN;
-  const float2 st = stats[row];
-  const float m = finite_or_zero(st.x), ks = k / st.y;
-  for (int c = threadIdx.x; c < n_cols; c += JTVAE_BLOCK) {
-    const float g = -ks * exp_nat((float)r[c] - m);
-    d[c] = (T)(c == label ? k + g : g);
+}
+
+enum { kStats = 0, kPolicy = 1 };
+
+// Whole rows in registers: RT lanes hold NV vectors of 16 bytes each, so a row is read once whatever is made of it.
+// kStats: statistics and log-probabilities of short rows.  kPolicy: the row's loss terms and, the coefficient of a policy
+// row depending on nothing else, its gradient in the same pass.  A block of RT * R threads owns R rows; the 64-bit
+// arithmetic of a row's end is done by one lane per row, side by side.
+template <typename T, int RT, int R, int NV, int MODE>
+__global__ __launch_bounds__(RT* R, NV > 8 ? 4 : 8) void rows_kernel(RowsIn<T> in, PolicyIn policy, float* __restrict__ coef,
+                                                     double* __restrict__ terms, GradOut<T> out) {
+  constexpr int E = Vec<T>::E, W = RT / 64;
+  __shared__ RowStat part[R * W];
+  __shared__ float4 end[R];  // m, s, coefficient, counted
+  const int r = threadIdx.x / RT, t = threadIdx.x % RT;
+  const int row = blockIdx.x * R + r;
+  const bool there = row < in.n_rows;
+  const long label = there ? in.labels[row] : -1;
+  const bool counted = there && counts(in, row, label);
+  const T* x = in.x + (long)row * in.ld;
+  const int n_vec = in.n_cols / E, c_tail = n_vec * E + t;
+  Word4 w[NV];
+  float tail = -INFINITY;
+  RowStat st = {-INFINITY, 0.f};
+  if (counted) {
+#pragma unroll
+    for (int u = 0; u < NV; ++u)
+      if (t + u * RT < n_vec) w[u] = Vec<T>::load(x + (long)(t + u * RT) * E);
+    if (c_tail < in.n_cols) tail = (float)x[c_tail];
+#pragma unroll
+    for (int u = 0; u < NV; ++u)
+      if (t + u * RT < n_vec) {
+        float v[E];
+        Vec<T>::unpack(w[u], v);
+        take<E>(st, v);
+      }
+    take<1>(st, &tail);
+    st = wave_join(st);
+    if ((t & 63) == 0) part[threadIdx.x >> 6] = st;
+  }
+  __syncthreads();
+  if (threadIdx.x < R) {
+    const int i = threadIdx.x, mine = blockIdx.x * R + i;
+    if (mine < in.n_rows) {
+      const long l = in.labels[mine];
+      const bool c = counts(in, mine, l);
+      RowStat s = {0.f, 1.f};
+      if (c) {
+        s = part[i * W];
+        for (int k = 1; k < W; ++k) s = join(s, part[i * W + k]);
+      }
+      const double lp = finish_row(in, mine, l, c, s);
+      if constexpr (MODE == kPolicy) {
+        PolicyRow p = {0.0, 0.0, 0.0, 0.f};
+        if (c) p = policy_row(policy, mine, lp);
+        coef[mine] = p.coef;
+        terms[3L * mine] = p.loss;
+        terms[3L * mine + 1] = p.kl;
+        terms[3L * mine + 2] = p.clipped;
+        end[i] = make_float4(s.m, s.s, l < in.n_cols ? p.coef : NAN, 0.f);
+      }
+    }
+  }
+  if constexpr (MODE == kPolicy) {
+    if (!out.dx) return;
+    __syncthreads();
+    if (!there) return;
+    T* d = out.dx + (long)row * out.ld;
+    const float4 f = end[r];
+    const float m = finite_or_zero(f.x), k = f.z, ks = k / f.y;
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+      const int i = t + u * RT;
+      if (i >= n_vec) break;
+      float v[E];
+      if (counted) {
+        Vec<T>::unpack(w[u], v);
+        softmax_grad<E>(v, (long)i * E, label, m, ks, k);
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = 0.f;
+      }
+      Vec<T>::store(d + (long)i * E, Vec<T>::pack(v));
+    }
+    if (c_tail < in.n_cols) {
+      float v = 0.f;
+      if (counted) {
+        v = tail;
+        softmax_grad<1>(&v, c_tail, label, m, ks, k);
+      }
+      d[c_tail] = (T)v;
+    }
+    for (long c = in.n_cols + t; c < out.width; c += RT) d[c] = (T)0.f;
+  }
+}
+
+// dx[row, j] = c ([j = label] - exp(x_j - m) / s), c = coef[owner or row] * upstream, from saved statistics.  Rows are
+// cut into tiles of RT lanes x NV vectors; a block of 256 threads owns 256 / RT tiles.  With unless_one the gradient
+// for an upstream factor of one is in place already and nothing is done where the factor is one.
+template <typename T, int RT, int NV>
+__global__ __launch_bounds__(JTVAE_BLOCK) void grad_kernel(RowsIn<T> in, const float* __restrict__ coef,
+                                                           const float* __restrict__ upstream, int unless_one,
+                                                           int tiles, GradOut<T> out) {
+  constexpr int E = Vec<T>::E;
+  const float up = upstream ? *upstream : 1.f;
+  if (unless_one && up == 1.f) return;
+  const long id = (long)blockIdx.x * (JTVAE_BLOCK / RT) + threadIdx.x / RT;
+  const int row = (int)(id / tiles), tile = (int)(id - (long)row * tiles), t = threadIdx.x % RT;
+  if (row >= in.n_rows) return;
+  const long label = in.labels[row];
+  const int own = in.owner ? in.owner[row] : row;
+  const bool counted = label >= 0 && own >= 0;
+  const T* x = in.x + (long)row * in.ld;
+  T* d = out.dx + (long)row * out.ld;
+  const int n_vec = in.n_cols / E, first = tile * RT * NV + t;
+  float k = 0.f, ks = 0.f, m = 0.f;
+  Word4 w[NV];
+  if (counted) {
+#pragma unroll
+    for (int u = 0; u < NV; ++u)
+      if (first + u * RT < n_vec) w[u] = Vec<T>::load(x + (long)(first + u * RT) * E);
+    const float2 st = in.stats[row];
+    k = label < in.n_cols ? coef[own] * up : NAN;
+    m = finite_or_zero(st.x);
+    ks = k / st.y;
+  }
+#pragma unroll
+  for (int u = 0; u < NV; ++u) {
+    const int i = first + u * RT;
+    if (i >= n_vec) break;
+    float v[E];
+    if (counted) {
+      Vec<T>::unpack(w[u], v);
+      softmax_grad<E>(v, (long)i * E, label, m, ks, k);
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[e] = 0.f;
+    }
+    Vec<T>::store(d + (long)i * E, Vec<T>::pack(v));
+  }
+  if (tile == tiles - 1) {  // columns after the last whole vector, and the padding
+    for (long c = (long)n_vec * E + t; c < out.width; c += RT) {
+      float v = 0.f;
+      if (counted && c < in.n_cols) {
+        v = (float)x[c];
+        softmax_grad<1>(&v, c, label, m, ks, k);
+      }
+      d[c] = (T)v;
+    }
   }
 }
 
@@ -195,38 +454,7 @@ __global__ __launch_bounds__(kPairBlock) void preference_pairs_kernel(
   }
 }
 
-// Policy rows: r = exp(lp - old), term = w (kl_coef k3 - min(r A, clip(r) A)), k3 = exp(ref - lp) - (ref - lp) - 1
-// (an unbiased, never negative estimate of the KL divergence from the sampled label alone), and
-// d term / d lp = w (kl_coef (1 - exp(ref - lp)) - [r A <= clip(r) A] r A).
-struct PolicyRow {
-  double loss, kl, clipped;
-  float coef;
-};
-
-struct PolicyIn {
-  const float *old_lp, *adv, *ref, *weights;
-  double lo, hi, kl_coef, scale;
-};
-
-__device__ __forceinline__ PolicyRow policy_row(const PolicyIn& in, int row, double lp) {
-  PolicyRow o;
-  const double w = in.scale * (in.weights ? (double)in.weights[row] : 1.0);
-  const double a = (double)in.adv[row], r = exp(lp - (double)in.old_lp[row]);
-  const double plain = r * a, cut = (r < in.lo ? in.lo : (r > in.hi ? in.hi : r)) * a;
-  const bool clipped = cut < plain;
-  double k3 = 0.0, dk3 = 0.0;
-  if (in.ref) {
-    const double gap = (double)in.ref[row] - lp, e = expm1(gap);
-    k3 = e - gap;
-    dk3 = -e;
-  }
-  o.loss = w * (in.kl_coef * k3 - (clipped ? cut : plain));
-  o.kl = w * k3;
-  o.clipped = clipped ? w : 0.0;
-  o.coef = (float)(w * (in.kl_coef * dk3 - (clipped ? 0.0 : plain)));
-  return o;
-}
-
+// Loss terms and coefficients of rows whose log-probabilities are there already.
 __global__ __launch_bounds__(JTVAE_BLOCK) void policy_rows_kernel(PolicyIn in, const double* __restrict__ lp64,
                                                                   Labels labels, int n_rows,
                                                                   float* __restrict__ coef,
@@ -274,19 +502,86 @@ int check_logits(const jtvae_logits_t* g) {
 }
 
 template <typename T>
+RowsIn<T> rows_in(const jtvae_logits_t* g, const int32_t* owner, float* stats, float* lp32, double* lp64) {
+  return RowsIn<T>{(const T*)g->x, (long)g->ld, g->n_rows, g->n_cols, Labels{g->labels, g->label_bits}, owner,
+                   (float2*)stats, lp32, lp64};
+}
+
+inline unsigned blocks_for(long items, int per) { return (unsigned)((items + per - 1) / per); }
+
+template <typename T, int RT, int R, int NV, int MODE>
+int launch_rows(const RowsIn<T>& in, const PolicyIn& p, float* coef, double* terms, const GradOut<T>& out,
+                hipStream_t s) {
+  hipLaunchKernelGGL((rows_kernel<T, RT, R, NV, MODE>), dim3(blocks_for(in.n_rows, R)), dim3(RT * R), 0, s, in, p, coef,
+                     terms, out);
+  return launch_status();
+}
+
+// Statistics.  Rows of up to 512 vectors (8 KiB) sit in a wave's registers, eight waves side by side; longer ones are
+// streamed by a block each: 256 threads where there are rows enough to fill the chip with them, 1024 where there are
+// not (a row of 128 000 bf16 then has all its loads in flight on one CU).
+template <typename T>
 int row_stats(const jtvae_logits_t* g, const int32_t* owner, float* stats, float* lp32, double* lp64, hipStream_t s) {
-  hipLaunchKernelGGL(row_stats_kernel<T>, dim3(g->n_rows), dim3(JTVAE_BLOCK), 0, s, (const T*)g->x, (long)g->ld,
-                     g->n_cols, Labels{g->labels, g->label_bits}, owner, (float2*)stats, lp32, lp64);
+  const RowsIn<T> in = rows_in<T>(g, owner, stats, lp32, lp64);
+  const int n_vec = g->n_cols / Vec<T>::E;
+  const PolicyIn none = {};
+  const GradOut<T> no_grad = {};
+  if (n_vec <= 128) return launch_rows<T, 64, 8, 2, kStats>(in, none, nullptr, nullptr, no_grad, s);
+  if (n_vec <= 512) return launch_rows<T, 64, 8, 8, kStats>(in, none, nullptr, nullptr, no_grad, s);
+  if (g->n_rows >= 1024)
+    hipLaunchKernelGGL((stats_kernel<T, 256>), dim3(g->n_rows), dim3(256), 0, s, in);
+  else
+    hipLaunchKernelGGL((stats_kernel<T, 1024>), dim3(g->n_rows), dim3(1024), 0, s, in);
+  return launch_status();
+}
+
+template <typename T, int RT, int NV>
+int launch_grad(const RowsIn<T>& in, const float* coef, const float* upstream, int unless_one, const GradOut<T>& out,
+                hipStream_t s) {
+  const int n_vec = in.n_cols / Vec<T>::E;
+  const int tiles = n_vec > RT * NV ? (n_vec + RT * NV - 1) / (RT * NV) : 1;
+  hipLaunchKernelGGL((grad_kernel<T, RT, NV>), dim3(blocks_for((long)in.n_rows * tiles, JTVAE_BLOCK / RT)),
+                     dim3(JTVAE_BLOCK), 0, s, in, coef, upstream, unless_one, tiles, out);
   return launch_status();
 }
 
 template <typename T>
 int row_grad(const jtvae_logits_t* g, const int32_t* owner, const float* stats, const float* coef,
-             const float* upstream, void* dx, int64_t ld_dx, int64_t width, hipStream_t s) {
-  hipLaunchKernelGGL(row_grad_kernel<T>, dim3(g->n_rows), dim3(JTVAE_BLOCK), 0, s, (const T*)g->x, (long)g->ld,
-                     g->n_cols, Labels{g->labels, g->label_bits}, owner, (const float2*)stats, coef, upstream, (T*)dx,
-                     (long)ld_dx, (long)width);
-  return launch_status();
+             const float* upstream, int unless_one, void* dx, int64_t ld_dx, int64_t width, hipStream_t s) {
+  const RowsIn<T> in = rows_in<T>(g, owner, (float*)stats, nullptr, nullptr);
+  const GradOut<T> out = {(T*)dx, (long)ld_dx, (long)width};
+  const int n_vec = g->n_cols / Vec<T>::E;
+  if (n_vec <= 128) return launch_grad<T, 64, 2>(in, coef, upstream, unless_one, out, s);
+  if (n_vec <= 256) return launch_grad<T, 64, 4>(in, coef, upstream, unless_one, out, s);
+  return launch_grad<T, 256, 4>(in, coef, upstream, unless_one, out, s);
+}
+
+// A policy row in one pass where its registers hold it; 1 when they do not.
+template <typename T>
+int policy_rows(const RowsIn<T>& in, const PolicyIn& p, float* coef, double* terms, const GradOut<T>& out,
+                hipStream_t s) {
+  const int n_vec = in.n_cols / Vec<T>::E;
+  if (n_vec <= 128) return launch_rows<T, 64, 8, 2, kPolicy>(in, p, coef, terms, out, s);
+  if (n_vec <= 512) return launch_rows<T, 64, 8, 8, kPolicy>(in, p, coef, terms, out, s);
+  if (n_vec <= 2048) return launch_rows<T, 256, 1, 8, kPolicy>(in, p, coef, terms, out, s);
+  if (n_vec <= 4096) return launch_rows<T, 512, 1, 8, kPolicy>(in, p, coef, terms, out, s);
+  if (n_vec <= 8192) return launch_rows<T, 1024, 1, 8, kPolicy>(in, p, coef, terms, out, s);
+  if (n_vec <= 16384) return launch_rows<T, 1024, 1, 16, kPolicy>(in, p, coef, terms, out, s);
+  return 1;
+}
+
+template <typename T>
+int policy(const jtvae_logits_t* g, const PolicyIn& in, float* stats, float* lp, float* coef, double* lp64,
+           double* terms, void* dx, int64_t ld_dx, int64_t width, hipStream_t s) {
+  const GradOut<T> out = {(T*)dx, (long)ld_dx, (long)width};
+  const int rc = policy_rows<T>(rows_in<T>(g, nullptr, stats, lp, nullptr), in, coef, terms, out, s);
+  if (rc != 1) return rc;
+  int e = row_stats<T>(g, nullptr, stats, lp, lp64, s);
+  if (e) return e;
+  hipLaunchKernelGGL(policy_rows_kernel, dim3(grid_for(g->n_rows)), dim3(JTVAE_BLOCK), 0, s, in, lp64,
+                     Labels{g->labels, g->label_bits}, g->n_rows, coef, terms);
+  e = launch_status();
+  return e || !dx ? e : row_grad<T>(g, nullptr, stats, coef, nullptr, 0, dx, ld_dx, width, s);
 }
 
 }  // namespace
@@ -313,18 +608,18 @@ int jtvae_label_log_probs(const jtvae_logits_t* logits, const int32_t* owner, fl
 }
 
 int jtvae_label_log_probs_bwd(const jtvae_logits_t* logits, const int32_t* owner, const float* stats,
-                              const float* coef, const float* upstream, void* dx, int64_t ld_dx, int64_t width,
-                              void* stream) {
+                              const float* coef, const float* upstream, int32_t unless_one, void* dx, int64_t ld_dx,
+                              int64_t width, void* stream) {
   JT_CHECK(check_logits(logits));
   if (width < logits->n_cols || ld_dx < width) return JTVAE_E_SHAPE;
   if (logits->n_rows == 0) return 0;
-  if (!stats || !coef || !dx) return JTVAE_E_NULL;
+  if (!stats || !coef || !dx || (unless_one && !upstream)) return JTVAE_E_NULL;
   if ((uintptr_t)dx % (logits->dtype == JTVAE_F32 ? 4 : 2)) return JTVAE_E_ALIGN;
   hipStream_t s = (hipStream_t)stream;
   switch (logits->dtype) {
-    case JTVAE_F32: return row_grad<float>(logits, owner, stats, coef, upstream, dx, ld_dx, width, s);
-    case JTVAE_F16: return row_grad<_Float16>(logits, owner, stats, coef, upstream, dx, ld_dx, width, s);
-    default: return row_grad<__bf16>(logits, owner, stats, coef, upstream, dx, ld_dx, width, s);
+    case JTVAE_F32: return row_grad<float>(logits, owner, stats, coef, upstream, unless_one, dx, ld_dx, width, s);
+    case JTVAE_F16: return row_grad<_Float16>(logits, owner, stats, coef, upstream, unless_one, dx, ld_dx, width, s);
+    default: return row_grad<__bf16>(logits, owner, stats, coef, upstream, unless_one, dx, ld_dx, width, s);
   }
 }
 
@@ -357,25 +652,34 @@ size_t jtvae_policy_loss_workspace_bytes(int32_t n_rows) {
 }
 
 int jtvae_policy_loss(const jtvae_logits_t* logits, const jtvae_policy_t* policy, float* stats, float* log_probs,
-                      float* coef, float* loss, float* kl, float* clipped, void* workspace, size_t workspace_bytes,
-                      void* stream) {
+                      float* coef, float* loss, float* kl, float* clipped, void* dx, int64_t ld_dx, int64_t width,
+                      void* workspace, size_t workspace_bytes, void* stream) {
   JT_CHECK(check_logits(logits));
   if (!policy || !loss || !kl || !clipped) return JTVAE_E_NULL;
   const int n = logits->n_rows;
   if (n > 0 && (!stats || !log_probs || !coef || !workspace || !policy->old_log_probs || !policy->advantages))
     return JTVAE_E_NULL;
+  if (dx && (width < logits->n_cols || ld_dx < width)) return JTVAE_E_SHAPE;
+  if ((uintptr_t)dx % (logits->dtype == JTVAE_F32 ? 4 : 2)) return JTVAE_E_ALIGN;
   if (workspace_bytes < jtvae_policy_loss_workspace_bytes(n)) return JTVAE_E_WORKSPACE;
   if (!(policy->clip_low >= 0.0 && policy->clip_low <= 1.0 && policy->clip_high >= 0.0)) return JTVAE_E_RANGE;
   hipStream_t s = (hipStream_t)stream;
   double* lp64 = (double*)workspace;
   double* terms = lp64 + n;
   if (n > 0) {
-    PolicyIn in = {policy->old_log_probs, policy->advantages, policy->ref_log_probs, policy->weights,
-                   1.0 - policy->clip_low, 1.0 + policy->clip_high, policy->kl_coef, policy->scale};
-    JT_CHECK(jtvae_label_log_probs(logits, nullptr, stats, log_probs, lp64, stream));
-    hipLaunchKernelGGL(policy_rows_kernel, dim3(grid_for(n)), dim3(JTVAE_BLOCK), 0, s, in, lp64,
-                       Labels{logits->labels, logits->label_bits}, n, coef, terms);
-    JT_CHECK(launch_status());
+    const PolicyIn in = {policy->old_log_probs, policy->advantages, policy->ref_log_probs, policy->weights,
+                         1.0 - policy->clip_low, 1.0 + policy->clip_high, policy->kl_coef, policy->scale};
+    int rc;
+    switch (logits->dtype) {
+      case JTVAE_F32:
+        rc = ::policy<float>(logits, in, stats, log_probs, coef, lp64, terms, dx, ld_dx, width, s);
+        break;
+      case JTVAE_F16:
+        rc = ::policy<_Float16>(logits, in, stats, log_probs, coef, lp64, terms, dx, ld_dx, width, s);
+        break;
+      default: rc = ::policy<__bf16>(logits, in, stats, log_probs, coef, lp64, terms, dx, ld_dx, width, s);
+    }
+    if (rc) return rc;
   }
   hipLaunchKernelGGL(sum_terms_kernel, dim3(1), dim3(kPairBlock), 0, s, terms, n, loss, kl, clipped);
   return launch_status();

@@ -263,12 +263,12 @@ SIGNATURES = {
     "jtvae_onehot_linear_bwd_workspace_bytes": (_sz, [_i32, _i32, _i32]),
     "jtvae_onehot_linear_bwd": (C.c_int, [_vp, _i32, _i32, _vp, _i32, _i32, _vp, _i32, _i32, _vp, _sz, _vp]),
     "jtvae_label_log_probs": (C.c_int, [C.POINTER(Logits), _vp, _vp, _vp, _vp, _vp]),
-    "jtvae_label_log_probs_bwd": (C.c_int, [C.POINTER(Logits), _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp]),
+    "jtvae_label_log_probs_bwd": (C.c_int, [C.POINTER(Logits), _vp, _vp, _vp, _vp, _i32, _vp, _i64, _i64, _vp]),
     "jtvae_sequence_sums": (C.c_int, [_vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp]),
     "jtvae_preference_pairs": (C.c_int, [_vp, _vp, _vp, _i32, _vp, _vp, _i32, _f64, _f64, _f64, _vp, _vp, _vp, _vp,
                                          _vp]),
     "jtvae_policy_loss_workspace_bytes": (_sz, [_i32]),
-    "jtvae_policy_loss": (C.c_int, [C.POINTER(Logits), C.POINTER(Policy), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "jtvae_policy_loss": (C.c_int, [C.POINTER(Logits), C.POINTER(Policy), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _sz, _vp]),
     "jtvae_grad_square_sums": (C.c_int, [C.POINTER(AdamwGroup), _vp, _vp]),
     "jtvae_grad_norm": (C.c_int, [_vp, _i64, _f64, _vp, _vp]),
     "jtvae_adamw_step": (C.c_int, [C.POINTER(AdamwGroup), _vp, _vp]),
@@ -700,9 +700,9 @@ def label_log_probs(g, owner, stats, log_probs, log_probs64):
          (C.byref(g), owner, stats, log_probs, log_probs64, stream_ptr()), nbytes=_logits_bytes(g) + 24 * g.n_rows)
 
 
-def label_log_probs_bwd(g, owner, stats, coef, upstream, dx, ld_dx, width):
+def label_log_probs_bwd(g, owner, stats, coef, upstream, dx, ld_dx, width, unless_one=False):
     _run("label_log_probs_bwd", lib.jtvae_label_log_probs_bwd,
-         (C.byref(g), owner, stats, coef, upstream, dx, ld_dx, width, stream_ptr()), nbytes=2 * _logits_bytes(g) + 20 * g.n_rows)
+         (C.byref(g), owner, stats, coef, upstream, int(unless_one), dx, ld_dx, width, stream_ptr()), nbytes=2 * _logits_bytes(g) + 20 * g.n_rows)
 
 
 def sequence_sums(log_probs64, rowptr, rows, n_seq, other, sums64, sums, n_rows=0):
@@ -721,10 +721,10 @@ def policy_loss_workspace_bytes(n_rows):
     return int(lib.jtvae_policy_loss_workspace_bytes(n_rows))
 
 
-def policy_loss(g, policy, stats, log_probs, coef, loss, kl, clipped, ws, ws_bytes):
+def policy_loss(g, policy, stats, log_probs, coef, loss, kl, clipped, dx, ld_dx, width, ws, ws_bytes):
     _run("policy_loss", lib.jtvae_policy_loss,
-         (C.byref(g), C.byref(policy), stats, log_probs, coef, loss, kl, clipped, ws, ws_bytes,
-          stream_ptr()), nbytes=_logits_bytes(g) + 40 * g.n_rows)
+         (C.byref(g), C.byref(policy), stats, log_probs, coef, loss, kl, clipped, dx, ld_dx, width, ws, ws_bytes,
+          stream_ptr()), nbytes=_logits_bytes(g) * (2 if dx else 1) + 40 * g.n_rows)
 
 
 def grad_square_sums(group, partials, n_elems=0):

@@ -174,11 +174,14 @@ def _arg(x, labels):
 def _like_rows(x):
     """(uninitialised gradient in the layout of ``x``, its leading dimension): the few padding columns of the package's
     row buffers are kept - the kernel writes them as zero - so that the products that follow take it without a copy."""
+    ld = _like_ld(x)
+    return torch.empty((x.shape[0], ld), dtype=x.dtype, device=x.device)[:, :x.shape[1]], ld
+
+
+def _like_ld(x):
     n, v = x.shape
     ld = x.stride(0) if n > 1 else v
-    if not v <= ld < v + 64:
-        ld = v
-    return torch.empty((n, ld), dtype=x.dtype, device=x.device)[:, :v], ld
+    return ld if v <= ld < v + 64 else v
 
 
 def _logits_grad(x, labels, owner, stats, coef, upstream):
@@ -334,9 +337,12 @@ class _PolicyLoss(torch.autograd.Function):
             ws = torch.empty((max(nbytes, 16),), dtype=torch.uint8, device=dev)
             g, keep = _arg(x, labels)
             policy = K.Policy(old.data_ptr(), adv.data_ptr(), K.ptr(ref), K.ptr(weights), lo, hi, kl_coef, scale)
+            # a row's coefficient depends on that row alone: its gradient is made while the row is in registers
+            d, ld = _like_rows(x) if ctx.needs_input_grad[0] else (None, 0)
             K.policy_loss(g, policy, stats.data_ptr(), lp.data_ptr(), coef.data_ptr(), loss.data_ptr(), kl.data_ptr(),
-                          clipped.data_ptr(), ws.data_ptr(), nbytes)
+                          clipped.data_ptr(), K.ptr(d), ld, ld, ws.data_ptr(), nbytes)
         ctx.save_for_backward(x if x.data_ptr() != logits.data_ptr() else logits, labels, stats, coef)
+        ctx.gradient = d
         ctx.mark_non_differentiable(lp, kl, clipped)
         ctx.set_materialize_grads(False)
         return loss, lp, kl, clipped
@@ -347,9 +353,17 @@ class _PolicyLoss(torch.autograd.Function):
         if dloss is None:
             return (None,) * 10
         logits, labels, stats, coef = ctx.saved_tensors
+        d, ctx.gradient = ctx.gradient, None
         with torch.cuda.device(logits.device):
             up = dloss.detach().float().contiguous()
-            d = _logits_grad(logits.detach(), labels, None, stats, coef, up)
+            x = logits.detach()
+            if d is None:  # a second pass through the graph: the first one's gradient has been given away
+                d = _logits_grad(x, labels, None, stats, coef, up)
+            else:  # stands as it is where the upstream factor is 1, which only the device knows
+                g, keep = _arg(x, labels)
+                ld = _like_ld(x)
+                K.label_log_probs_bwd(g, None, stats.data_ptr(), coef.data_ptr(), up.data_ptr(), d.data_ptr(), ld, ld,
+                                      unless_one=True)
         return (d,) + (None,) * 9
 
 

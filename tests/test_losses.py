@@ -114,10 +114,11 @@ def test_c_entry_points_refuse_before_launch():
     assert lp(K.logits_arg(258, 8, 4, 7, K.BF16, 260, 64)) == K.E_ALIGN
     assert lp(K.logits_arg(None, 8, 0, 7, K.F32, None, 64)) == 0  # no rows: nothing to do
     bwd = lib.jtvae_label_log_probs_bwd
-    assert bwd(ctypes.byref(ok), None, 256, 256, None, 256, 7, 8, None) == K.E_SHAPE  # width > ld_dx
-    assert bwd(ctypes.byref(ok), None, 256, 256, None, 256, 8, 6, None) == K.E_SHAPE  # width < n_cols
-    assert bwd(ctypes.byref(ok), None, 256, 256, None, 257, 8, 8, None) == K.E_ALIGN
-    assert bwd(ctypes.byref(ok), None, None, 256, None, 256, 8, 8, None) == K.E_NULL
+    assert bwd(ctypes.byref(ok), None, 256, 256, None, 0, 256, 7, 8, None) == K.E_SHAPE  # width > ld_dx
+    assert bwd(ctypes.byref(ok), None, 256, 256, None, 0, 256, 8, 6, None) == K.E_SHAPE  # width < n_cols
+    assert bwd(ctypes.byref(ok), None, 256, 256, None, 0, 257, 8, 8, None) == K.E_ALIGN
+    assert bwd(ctypes.byref(ok), None, None, 256, None, 0, 256, 8, 8, None) == K.E_NULL
+    assert bwd(ctypes.byref(ok), None, 256, 256, None, 1, 256, 8, 8, None) == K.E_NULL  # unless_one without upstream
     assert lib.jtvae_sequence_sums(None, None, None, 0, None, None, None, None) == 0
     assert lib.jtvae_sequence_sums(None, 256, 256, 2, None, None, 256, None) == K.E_NULL
     assert lib.jtvae_sequence_sums(256, 256, 256, -2, None, None, 256, None) == K.E_SHAPE
@@ -129,7 +130,7 @@ def test_c_entry_points_refuse_before_launch():
     assert need > 0 and K.policy_loss_workspace_bytes(0) == 0
 
     def policy(p=pol, g=ok, ws=need, stats=256, loss=256):
-        return lib.jtvae_policy_loss(ctypes.byref(g), ctypes.byref(p), stats, 256, 256, loss, 256, 256, 256, ws, None)
+        return lib.jtvae_policy_loss(ctypes.byref(g), ctypes.byref(p), stats, 256, 256, loss, 256, 256, None, 0, 0, 256, ws, None)
 
     assert policy(ws=need - 1) == K.E_WORKSPACE and policy(stats=None) == K.E_NULL and policy(loss=None) == K.E_NULL
     assert policy(p=K.Policy(None, 256, None, None, 0.2, 0.2, 0.0, 1.0)) == K.E_NULL
