@@ -535,25 +535,42 @@ int jtvae_label_log_probs(const jtvae_logits_t* logits, const int32_t* owner, fl
 
 /* dx[i, j] = c_i ([j = label_i] - softmax(x_i)_j) in the logits' type, c_i = coef[owner ? owner[i] : i] * upstream
  * (device scalar, or NULL = 1); rows without a label get zeros.  Columns [n_cols, width) are padding and
- * become zero (n_cols <= width <= ld_dx).  unless_one: dx holds the gradient for upstream = 1 already, nothing is done
- * if *upstream is 1. */
+ * become zero (n_cols <= width <= ld_dx).  unless_one: dx holds the gradient for upstream = 1 already and stays
+ * as it is if *upstream is 1.  scaled (n_scaled > 0): scaled[q] = coef[q] * upstream. */
 int jtvae_label_log_probs_bwd(const jtvae_logits_t* logits, const int32_t* owner, const float* stats,
                               const float* coef, const float* upstream, int32_t unless_one, void* dx, int64_t ld_dx,
-                              int64_t width, void* stream);
+                              int64_t width, float* scaled, int32_t n_scaled, void* stream);
 
-/* sums[q] = sum of log_probs64 over rows[rowptr[q] .. rowptr[q+1]) (+ other[q]); sums64: the same unrounded, or
- * NULL.  Fixed order: bitwise reproducible. */
-int jtvae_sequence_sums(const double* log_probs64, const int32_t* rowptr, const int32_t* rows, int32_t n_seq,
-                        const float* other, double* sums64, float* sums, void* stream);
+/* Which sequence every row belongs to, and pairs of sequences (device tables). */
+typedef struct jtvae_sequences {
+  const int32_t* row_seq;   /* [n_rows] sequence of every row, < 0: none                                */
+  const int32_t* rowptr;    /* [n_seq + 1], rows: the same as CSR                                       */
+  const int32_t* rows;
+  int32_t n_seq;
+  const int32_t* pairs;     /* [n_pairs, 2] (preferred, other) sequence                                 */
+  int32_t n_pairs;
+  const int32_t* pair_ptr;  /* [n_seq + 1], pair_list: the pairs that name a sequence, as 2 pair + side */
+  const int32_t* pair_list;
+} jtvae_sequences_t;
 
-/* pairs[p] = (preferred, other) sequence.  margin_p = beta ((sums64 - ref)[preferred] - (sums64 - ref)[other]);
- * loss = scale * sum_p -(1 - smoothing) log sigmoid(margin_p) - smoothing log sigmoid(-margin_p);
- * coef[q] = d loss / d sums64[q].  seq_ptr / seq_pairs: CSR of the pairs that name sequence q, as 2 p + side.
- * dmargin: scratch [n_pairs]. */
-int jtvae_preference_pairs(const double* sums64, const float* ref, const int32_t* pairs, int32_t n_pairs,
-                           const int32_t* seq_ptr, const int32_t* seq_pairs, int32_t n_seq, double beta,
-                           double smoothing, double scale, float* loss, float* margins, double* dmargin, float* coef,
-                           void* stream);
+/* sums[q] = sum of the rows' label log-probabilities per sequence, added in 64 bits in a fixed order. */
+size_t jtvae_sequence_log_probs_workspace_bytes(int32_t n_rows);
+int jtvae_sequence_log_probs(const jtvae_logits_t* logits, const jtvae_sequences_t* sequences, float* stats,
+                             float* sums, void* workspace, size_t workspace_bytes, void* stream);
+
+typedef struct jtvae_preference {
+  const float* ref_log_probs;   /* [n_seq] log-probability under the reference model                    */
+  const float* other_log_probs; /* [n_seq] terms from outside the logits, or NULL                       */
+  double beta, label_smoothing, scale;
+} jtvae_preference_t;
+
+/* With S the sequences' sums (other_log_probs included): margin_p = beta ((S - ref)[preferred] - (S - ref)[other]),
+ * loss = scale * sum_p -(1 - label_smoothing) log sigmoid(margin_p) - label_smoothing log sigmoid(-margin_p);
+ * coef[q] = d loss / d S_q, which with row_seq as owner is what jtvae_label_log_probs_bwd takes. */
+size_t jtvae_preference_loss_workspace_bytes(int32_t n_rows, int32_t n_seq, int32_t n_pairs);
+int jtvae_preference_loss(const jtvae_logits_t* logits, const jtvae_sequences_t* sequences,
+                          const jtvae_preference_t* preference, float* stats, float* sums, float* margins,
+                          float* coef, float* loss, void* workspace, size_t workspace_bytes, void* stream);
 
 typedef struct jtvae_policy {
   const float* old_log_probs; /* [n_rows] log-probability of the label when it was sampled             */
@@ -579,7 +596,8 @@ int jtvae_policy_loss(const jtvae_logits_t* logits, const jtvae_policy_t* policy
 #define JTVAE_ADAMW_CHUNK 4096       /* elements of a tensor one workgroup updates                          */
 #define JTVAE_ADAMW_MAX_TENSORS 400  /* gradient addresses one launch carries; longer lists take several    */
 
-/* One parameter tensor, contiguous; this table is DEVICE memory.  States start at 16-byte boundaries. */
+/* One parameter tensor, contiguous; this table is DEVICE memory.  States start at 16-byte boundaries; 8-bit ones are
+ * allocated up to whole blocks of JTVAE_ADAMW_BLOCK elements. */
 typedef struct jtvae_adamw_tensor {
   void* param;         /* dtype of the group                                                        */
   float* master;       /* fp32 copy the step works on (16-bit parameters), or NULL                  */
@@ -606,21 +624,17 @@ typedef struct jtvae_adamw_group {
   double lr, beta1, beta2, eps, weight_decay;
 } jtvae_adamw_group_t;
 
-/* partials[c] = sum of squares of the gradient elements of chunk c (0 where there is no gradient), [n_chunks]. */
-int jtvae_grad_square_sums(const jtvae_adamw_group_t* group, double* partials, void* stream);
-
-/* norm[0] = sqrt(sum of partials), norm[1] = min(1, max_norm / (norm[0] + 1e-6)): what every gradient is multiplied by
- * to bring their common 2-norm down to max_norm. */
-int jtvae_grad_norm(const double* partials, int64_t n_partials, double max_norm, float* norm, void* stream);
-
-/* One step of the tensors that have a gradient.  g = grad * *grad_scale (device scalar, or NULL = 1), t = ++steps:
+/* One step of the tensors that have a gradient, over all groups.  With max_norm > 0 every gradient is multiplied by
+ * norm[1] = min(1, max_norm / (norm[0] + 1e-6)), norm[0] being the 2-norm of all of them (device [2]; partials: scratch, a
+ * double per chunk of all groups together); max_norm = 0: as they are.  With t = ++steps,
  *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
  *   w = w (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
  * on the fp32 copy where there is one, whose rounded value then becomes the parameter.  8-bit states hold m and
  * sqrt(v) as e4m3 values times the block's scale max / 448, rounded to nearest after the update; a root that is not
  * zero keeps at least the smallest value 2^-9, so that it never leaves m divided by eps alone.  A maximum of at most
  * 2^-100 counts as zero.  An element that is not finite becomes NaN and leaves the rest of its block as it is. */
-int jtvae_adamw_step(const jtvae_adamw_group_t* group, const float* grad_scale, void* stream);
+int jtvae_adamw_step(const jtvae_adamw_group_t* groups, int32_t n_groups, double max_norm, double* partials,
+                     float* norm, void* stream);
 
 /* ---- host-side index preparation (host memory in and out; no GPU work, no stream) ---------- */
 

@@ -1,19 +1,19 @@
 // AdamW over many tensors at once: one launch for all tensors of a group, states in fp32 or in 8 bits with a scale per
 // 256 elements, and the global 2-norm of the gradients that the step multiplies them down to.
 //
-// A workgroup owns one chunk of one tensor (the chunk list is built once); a wave owns whole 256-element blocks of it,
-// four elements a lane, so that a block's scale is one wave reduction.  The addresses of the gradients, which change
-// from step to step, travel with the launch.
+// A workgroup owns one chunk of one tensor (the chunk list is built once), a wave whole 256-element blocks of it, so that
+// a block's scale is a reduction over neighbouring lanes.  The addresses of the gradients, which change from step to
+// step, travel with the launch.
 #include "../../include/jtvae_hip.h"
 #include "jtvae_common.h"
 
 namespace {
 
 constexpr int kBlock = 256;                   // threads of a workgroup
-constexpr int kGroup = JTVAE_ADAMW_BLOCK;     // elements that share a scale: 64 lanes x 4
+constexpr int kGroup = JTVAE_ADAMW_BLOCK;     // elements that share a scale
 constexpr float kSmallest = 0x1p-100f;        // maxima up to this count as zero
 constexpr float kTop = 448.f;                 // largest e4m3 value
-static_assert(kGroup == 256 && JTVAE_ADAMW_CHUNK % (kBlock * 4) == 0, "a wave owns whole blocks");
+static_assert(kGroup == 256 && JTVAE_ADAMW_CHUNK % kGroup == 0, "a wave owns whole blocks");
 
 struct Grads {
   const void* at[JTVAE_ADAMW_MAX_TENSORS];
@@ -25,16 +25,51 @@ inline int launch_status() {
   return e == hipSuccess ? 0 : (int)e;
 }
 
-template <typename T>
-__device__ __forceinline__ void load4(const T* p, long i, long n, float v[4]) {
+// N consecutive elements from i, at the type's own alignment (the hardware takes a 16-byte access at any address); WHOLE:
+// all of them exist, else those from n on read as zero and are not written.
+template <typename T, int N>
+struct __attribute__((packed, aligned(sizeof(T)))) Run {
+  T at[N];
+};
+
+template <bool WHOLE, int N, typename T>
+__device__ __forceinline__ void load(const T* p, long i, long n, float v[N]) {
+  if constexpr (WHOLE) {
+    const Run<T, N> r = *(const Run<T, N>*)(p + i);
 #pragma unroll
-  for (int k = 0; k < 4; ++k) v[k] = i + k < n ? (float)p[i + k] : 0.f;
+    for (int k = 0; k < N; ++k) v[k] = (float)r.at[k];
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] = i + k < n ? (float)p[i + k] : 0.f;
+  }
 }
-template <typename T>
-__device__ __forceinline__ void store4(T* p, long i, long n, const float v[4]) {
+template <bool WHOLE, int N, typename T>
+__device__ __forceinline__ void store(T* p, long i, long n, const float v[N]) {
+  if constexpr (WHOLE) {
+    Run<T, N> r;
 #pragma unroll
-  for (int k = 0; k < 4; ++k)
-    if (i + k < n) p[i + k] = (T)v[k];
+    for (int k = 0; k < N; ++k) r.at[k] = (T)v[k];
+    *(Run<T, N>*)(p + i) = r;
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (i + k < n) p[i + k] = (T)v[k];
+  }
+}
+
+template <bool WHOLE, typename T>
+__device__ __forceinline__ double chunk_squares(const T* g, long base, long n) {
+  constexpr int N = 16 / sizeof(T);
+  double acc = 0.0;
+#pragma unroll
+  for (int u = 0; u < JTVAE_ADAMW_CHUNK / (kBlock * N); ++u) {
+    float v[N], s = 0.f;
+    load<WHOLE, N>(g, base + (u * kBlock + threadIdx.x) * N, n, v);
+#pragma unroll
+    for (int k = 0; k < N; ++k) s = fmaf(v[k], v[k], s);
+    acc += (double)s;
+  }
+  return acc;
 }
 
 template <typename T>
@@ -48,11 +83,7 @@ __global__ __launch_bounds__(kBlock) void square_sums_kernel(const jtvae_adamw_t
   double acc = 0.0;
   if (g) {
     const long n = tensors[c.x].n, base = (long)c.y * JTVAE_ADAMW_CHUNK;
-    for (int i = threadIdx.x * 4; i < JTVAE_ADAMW_CHUNK; i += kBlock * 4) {
-      float v[4];
-      load4(g, base + i, n, v);
-      acc += (double)(v[0] * v[0] + v[1] * v[1] + v[2] * v[2] + v[3] * v[3]);
-    }
+    acc = base + JTVAE_ADAMW_CHUNK <= n ? chunk_squares<true>(g, base, n) : chunk_squares<false>(g, base, n);
   }
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) acc += __shfl_xor(acc, off, 64);
@@ -61,40 +92,50 @@ __global__ __launch_bounds__(kBlock) void square_sums_kernel(const jtvae_adamw_t
   if (threadIdx.x == 0) partials[chunk] = part[0] + part[1] + part[2] + part[3];
 }
 
-constexpr int kNormBlock = 1024;
-
-__global__ __launch_bounds__(kNormBlock) void grad_norm_kernel(const double* __restrict__ partials, long n,
-                                                               double max_norm, float* __restrict__ norm) {
-  __shared__ double part[kNormBlock / 64];
-  double acc = 0.0;
-  for (long i = threadIdx.x; i < n; i += kNormBlock) acc += partials[i];
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) acc += __shfl_xor(acc, off, 64);
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = acc;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    double t = 0.0;
-    for (int w = 0; w < kNormBlock / 64; ++w) t += part[w];
-    t = sqrt(t);
-    const double coef = max_norm / (t + 1e-6);
-    norm[0] = (float)t;
-    norm[1] = coef < 1.0 ? (float)coef : (coef == coef ? 1.f : (float)coef);  // a NaN norm stays visible
-  }
-}
+constexpr int kPrepBlock = 1024;
+static_assert(JTVAE_ADAMW_MAX_TENSORS <= kPrepBlock, "one thread per tensor");
 
 struct Present {
   unsigned bits[(JTVAE_ADAMW_MAX_TENSORS + 31) / 32];
   int first, count;
 };
 
-// t = ++steps of the tensors that have a gradient; bias = (1 / (1 - beta1^t), 1 / sqrt(1 - beta2^t)), in fp64.
-__global__ __launch_bounds__(kBlock) void steps_kernel(int* __restrict__ steps, float2* __restrict__ bias,
-                                                       Present present, double beta1, double beta2) {
-  const int i = blockIdx.x * kBlock + threadIdx.x;
-  if (i >= present.count || !(present.bits[i >> 5] >> (i & 31) & 1)) return;
-  const int t = ++steps[present.first + i];
-  bias[present.first + i] =
-      make_float2((float)(1.0 / (1.0 - pow(beta1, (double)t))), (float)(1.0 / sqrt(1.0 - pow(beta2, (double)t))));
+struct Norm {
+  const double* partials;
+  long n;
+  double max_norm;
+  float* out;
+};
+
+// What the update needs before it starts.  Block 0: t = ++steps of the tensors that have a gradient and their bias
+// corrections (1 / (1 - beta1^t), 1 / sqrt(1 - beta2^t)), formed in fp64.  Block 1, where the gradients are clipped: the
+// norm from the chunks' sums in a fixed order, and the factor min(1, max_norm / (norm + 1e-6)).
+__global__ __launch_bounds__(kPrepBlock) void prepare_kernel(int* __restrict__ steps, float2* __restrict__ bias,
+                                                             Present present, double beta1, double beta2, Norm norm) {
+  __shared__ double part[kPrepBlock / 64];
+  const int i = threadIdx.x;
+  if (blockIdx.x == 0) {
+    if (i >= present.count || !(present.bits[i >> 5] >> (i & 31) & 1)) return;
+    const int t = ++steps[present.first + i];
+    bias[present.first + i] = make_float2((float)(1.0 / (1.0 - pow(beta1, (double)t))),
+                                          (float)(1.0 / sqrt(1.0 - pow(beta2, (double)t))));
+    return;
+  }
+  double acc = 0.0;
+#pragma unroll 8
+  for (long k = i; k < norm.n; k += kPrepBlock) acc += norm.partials[k];
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) acc += __shfl_xor(acc, off, 64);
+  if ((i & 63) == 0) part[i >> 6] = acc;
+  __syncthreads();
+  if (i == 0) {
+    double t = 0.0;
+    for (int w = 0; w < kPrepBlock / 64; ++w) t += part[w];
+    t = sqrt(t);
+    const double coef = norm.max_norm / (t + 1e-6);
+    norm.out[0] = (float)t;
+    norm.out[1] = coef < 1.0 ? (float)coef : (coef == coef ? 1.f : (float)coef);  // a NaN norm stays visible
+  }
 }
 
 struct Hyper {
@@ -102,49 +143,157 @@ struct Hyper {
   const float *lr_device, *grad_scale;
 };
 
-// Four e4m3 values of one 32-bit word, and back with the format's rounding to nearest even.
-__device__ __forceinline__ void unpack_e4m3(unsigned w, float v[4]) {
-  auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
-  v[0] = lo[0];
-  v[1] = lo[1];
-  v[2] = hi[0];
-  v[3] = hi[1];
-}
-__device__ __forceinline__ unsigned pack_e4m3(const float v[4]) {
-  int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
-  w = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], w, true);
-  return (unsigned)w;
-}
-
-__device__ __forceinline__ float wave_max(float v) {
+// e4m3 values of a lane, four to a 32-bit word, and back with the format's rounding to nearest even.
+template <int N>
+__device__ __forceinline__ void unpack_e4m3(const uint8_t q[N], float v[N]) {
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
-  return v;
+  for (int k = 0; k < N; k += 4) {
+    int w;
+    __builtin_memcpy(&w, q + k, 4);
+    auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
+    v[k] = lo[0];
+    v[k + 1] = lo[1];
+    v[k + 2] = hi[0];
+    v[k + 3] = hi[1];
+  }
+}
+template <int N>
+__device__ __forceinline__ void pack_e4m3(const float v[N], uint8_t q[N]) {
+#pragma unroll
+  for (int k = 0; k < N; k += 4) {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[k], v[k + 1], 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(v[k + 2], v[k + 3], w, true);
+    __builtin_memcpy(q + k, &w, 4);
+  }
 }
 
-// Largest finite magnitude of a wave's 256 values: the scale is not lost to one element that overflowed.
-__device__ __forceinline__ float block_top(const float v[4]) {
+// Largest finite magnitude among the values of the lanes that share a scale: a scale is not lost to one element that
+// overflowed.
+template <int N>
+__device__ __forceinline__ float block_top(const float v[N]) {
   float t = 0.f;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
+  for (int k = 0; k < N; ++k) {
     const float a = fabsf(v[k]);
-    if (a < INFINITY) t = fmaxf(t, a);
+    t = fmaxf(t, a < INFINITY ? a : 0.f);
   }
-  return wave_max(t);
+#pragma unroll
+  for (int off = kGroup / N / 2; off > 0; off >>= 1) t = fmaxf(t, __shfl_xor(t, off, 64));
+  return t;
 }
 
-template <bool ROOT>
-__device__ __forceinline__ unsigned quantise(const float v[4], float top) {
+template <bool ROOT, int N>
+__device__ __forceinline__ void quantise(const float v[N], float top, uint8_t q[N]) {
   const float inv = top > kSmallest ? kTop / top : 0.f;
-  float q[4];
+  float x[N];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    q[k] = v[k] * inv;
-    if (ROOT && q[k] > 0.f) q[k] = fmaxf(q[k], 0x1p-9f);
-    if (!(fabsf(v[k]) < INFINITY)) q[k] = NAN;
-    else q[k] = fminf(fmaxf(q[k], -kTop), kTop);
+  for (int k = 0; k < N; ++k) {
+    float y = fminf(fmaxf(v[k] * inv, -kTop), kTop);
+    if (ROOT) y = y > 0.f ? fmaxf(y, 0x1p-9f) : y;
+    x[k] = fabsf(v[k]) < INFINITY ? y : NAN;
   }
-  return pack_e4m3(q);
+  pack_e4m3<N>(x, q);
+}
+
+// sqrt on the hardware unit (1 ulp), with what it would flush brought into its range first.
+__device__ __forceinline__ float root(float v) {
+  const bool low = v < 0x1p-96f;
+  const float r = __builtin_amdgcn_sqrtf(low ? v * 0x1p96f : v);
+  return low ? r * 0x1p-48f : r;
+}
+
+struct Step {
+  float keep, rate, eps, beta1, one_m_beta1, beta2, one_m_beta2, grad_scale, bias2;
+};
+
+// N elements of a tensor from `at`: loads, the update, and what goes back.  8-bit states: kGroup / N neighbouring lanes
+// share a scale.
+template <typename T, bool MASTER, int BITS, bool WHOLE, int N>
+struct Piece {
+  float g[N], w[N], m[N], v[N];
+  uint8_t qm[N], qr[N];
+  float sm, sr;
+
+  __device__ __forceinline__ void fetch(const jtvae_adamw_tensor_t& t, const T* grad, long at) {
+    load<WHOLE, N>(grad, at, t.n, g);
+    if constexpr (MASTER) load<WHOLE, N>((const float*)t.master, at, t.n, w);
+    else load<WHOLE, N>((const T*)t.param, at, t.n, w);
+    if constexpr (BITS == 32) {
+      load<WHOLE, N>((const float*)t.exp_avg, at, t.n, m);
+      load<WHOLE, N>((const float*)t.second, at, t.n, v);
+    } else {
+      // the states' buffers are padded to whole blocks
+      __builtin_memcpy(qm, __builtin_assume_aligned((const uint8_t*)t.exp_avg + at, N), N);
+      __builtin_memcpy(qr, __builtin_assume_aligned((const uint8_t*)t.second + at, N), N);
+      sm = t.exp_avg_scale[at / kGroup];
+      sr = t.second_scale[at / kGroup];
+    }
+  }
+
+  __device__ __forceinline__ void update(const jtvae_adamw_tensor_t& t, const Step& s, long at) {
+    float r[N];
+    if constexpr (BITS == 8) {
+      unpack_e4m3<N>(qm, m);
+      unpack_e4m3<N>(qr, r);
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        m[k] *= sm;
+        r[k] *= sr;
+        v[k] = r[k] * r[k];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const float x = g[k] * s.grad_scale;
+      m[k] = s.beta1 * m[k] + s.one_m_beta1 * x;
+      v[k] = s.beta2 * v[k] + s.one_m_beta2 * (x * x);
+      r[k] = root(v[k]);
+      // reciprocal on the hardware unit (1 ulp): the update is off by 2^-22 of itself, below half an ulp of w
+      w[k] = w[k] * s.keep - s.rate * (m[k] * __builtin_amdgcn_rcpf(r[k] * s.bias2 + s.eps));
+    }
+    if constexpr (MASTER) store<WHOLE, N>(t.master, at, t.n, w);
+    store<WHOLE, N>((T*)t.param, at, t.n, w);
+    if constexpr (BITS == 32) {
+      store<WHOLE, N>((float*)t.exp_avg, at, t.n, m);
+      store<WHOLE, N>((float*)t.second, at, t.n, v);
+    } else {
+      if constexpr (!WHOLE) {  // the padding after the last element stays zero
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+          if (at + k >= t.n) m[k] = r[k] = 0.f;
+      }
+      const float tm = block_top<N>(m), tr = block_top<N>(r);
+      quantise<false, N>(m, tm, qm);
+      quantise<true, N>(r, tr, qr);
+      __builtin_memcpy(__builtin_assume_aligned((uint8_t*)t.exp_avg + at, N), qm, N);
+      __builtin_memcpy(__builtin_assume_aligned((uint8_t*)t.second + at, N), qr, N);
+      if ((threadIdx.x & (kGroup / N - 1)) == 0) {
+        t.exp_avg_scale[at / kGroup] = tm > kSmallest ? tm / kTop : 0.f;
+        t.second_scale[at / kGroup] = tr > kSmallest ? tr / kTop : 0.f;
+      }
+    }
+  }
+};
+
+template <typename T, bool MASTER, int BITS, bool WHOLE>
+__device__ __forceinline__ void update_chunk(const jtvae_adamw_tensor_t& t, const T* g, long base, const Step& s) {
+  constexpr int N = BITS == 8 ? 8 : 4, U = 2, kStride = kBlock * N;
+  static_assert(JTVAE_ADAMW_CHUNK % (kStride * U) == 0, "whole rounds");
+#pragma unroll
+  for (int i = 0; i < JTVAE_ADAMW_CHUNK; i += kStride * U) {
+    Piece<T, MASTER, BITS, WHOLE, N> p[U];
+    bool there[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const long at = base + i + u * kStride + threadIdx.x * N;
+      // the same for all lanes that share a scale: the first element of their block
+      there[u] = WHOLE || at / kGroup * kGroup < t.n;
+      if (there[u]) p[u].fetch(t, g, at);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (there[u]) p[u].update(t, s, base + i + u * kStride + threadIdx.x * N);
+  }
 }
 
 template <typename T, bool MASTER, int BITS>
@@ -157,65 +306,11 @@ __global__ __launch_bounds__(kBlock) void adamw_kernel(const jtvae_adamw_tensor_
   const jtvae_adamw_tensor_t t = tensors[c.x];
   const float2 b = bias[c.x];
   const float lr = h.lr_device ? *h.lr_device : h.lr;
-  const float gs = h.grad_scale ? *h.grad_scale : 1.f;
-  const float keep = 1.f - lr * h.decay, rate = lr * b.x;
+  const Step s = {1.f - lr * h.decay, lr * b.x,      h.eps, h.beta1, h.one_m_beta1, h.beta2, h.one_m_beta2,
+                  h.grad_scale ? *h.grad_scale : 1.f, b.y};
   const long base = (long)c.y * JTVAE_ADAMW_CHUNK;
-  const int lane = threadIdx.x & 63;
-  for (int i = threadIdx.x * 4; i < JTVAE_ADAMW_CHUNK; i += kBlock * 4) {
-    const long at = base + i;
-    if (at - lane * 4 >= t.n) break;  // the same for every lane of a wave: its first element
-    float gv[4], w[4], m[4], v[4], r[4];
-    load4(g, at, t.n, gv);
-    if (MASTER) load4(t.master, at, t.n, w);
-    else load4((const T*)t.param, at, t.n, w);
-    if constexpr (BITS == 32) {
-      load4((const float*)t.exp_avg, at, t.n, m);
-      load4((const float*)t.second, at, t.n, v);
-    } else {
-      const long blk = at / kGroup;
-      const float sm = t.exp_avg_scale[blk], sr = t.second_scale[blk];
-      unsigned qm = 0, qr = 0;
-      for (int k = 0; k < 4; ++k)
-        if (at + k < t.n) {
-          qm |= (unsigned)((const uint8_t*)t.exp_avg)[at + k] << (8 * k);
-          qr |= (unsigned)((const uint8_t*)t.second)[at + k] << (8 * k);
-        }
-      unpack_e4m3(qm, m);
-      unpack_e4m3(qr, r);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        m[k] *= sm;
-        r[k] *= sr;
-        v[k] = r[k] * r[k];
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float x = gv[k] * gs;
-      m[k] = h.beta1 * m[k] + h.one_m_beta1 * x;
-      v[k] = h.beta2 * v[k] + h.one_m_beta2 * (x * x);
-      r[k] = sqrtf(v[k]);
-      w[k] = w[k] * keep - rate * (m[k] / (r[k] * b.y + h.eps));
-    }
-    if (MASTER) store4(t.master, at, t.n, w);
-    store4((T*)t.param, at, t.n, w);
-    if constexpr (BITS == 32) {
-      store4((float*)t.exp_avg, at, t.n, m);
-      store4((float*)t.second, at, t.n, v);
-    } else {
-      const float tm = block_top(m), tr = block_top(r);
-      const unsigned qm = quantise<false>(m, tm), qr = quantise<true>(r, tr);
-      for (int k = 0; k < 4; ++k)
-        if (at + k < t.n) {
-          ((uint8_t*)t.exp_avg)[at + k] = (uint8_t)(qm >> (8 * k));
-          ((uint8_t*)t.second)[at + k] = (uint8_t)(qr >> (8 * k));
-        }
-      if (lane == 0) {
-        t.exp_avg_scale[at / kGroup] = tm > kSmallest ? tm / kTop : 0.f;
-        t.second_scale[at / kGroup] = tr > kSmallest ? tr / kTop : 0.f;
-      }
-    }
-  }
+  if (base + JTVAE_ADAMW_CHUNK <= t.n) update_chunk<T, MASTER, BITS, true>(t, g, base, s);
+  else update_chunk<T, MASTER, BITS, false>(t, g, base, s);
 }
 
 int check_group(const jtvae_adamw_group_t* g) {
@@ -276,53 +371,62 @@ int square_sums(const jtvae_adamw_group_t* g, double* partials, hipStream_t s) {
 
 extern "C" {
 
-int jtvae_grad_square_sums(const jtvae_adamw_group_t* group, double* partials, void* stream) {
-  JT_CHECK(check_group(group));
-  if (group->n_chunks == 0) return 0;
-  if (!partials) return JTVAE_E_NULL;
+int jtvae_adamw_step(const jtvae_adamw_group_t* groups, int32_t n_groups, double max_norm, double* partials,
+                     float* norm, void* stream) {
+  if (n_groups < 0) return JTVAE_E_SHAPE;
+  if (n_groups && !groups) return JTVAE_E_NULL;
+  if (!(max_norm >= 0.0)) return JTVAE_E_RANGE;
+  if (max_norm > 0.0 && (!partials || !norm)) return JTVAE_E_NULL;
+  for (int i = 0; i < n_groups; ++i) {
+    const jtvae_adamw_group_t& g = groups[i];
+    JT_CHECK(check_group(&g));
+    if (!(g.beta1 >= 0.0 && g.beta1 < 1.0 && g.beta2 >= 0.0 && g.beta2 < 1.0 && g.eps >= 0.0)) return JTVAE_E_RANGE;
+    if (g.n_tensors && (!g.steps || !g.bias)) return JTVAE_E_NULL;
+  }
   hipStream_t s = (hipStream_t)stream;
-  switch (group->dtype) {
-    case JTVAE_F32: return square_sums<float>(group, partials, s);
-    case JTVAE_F16: return square_sums<_Float16>(group, partials, s);
-    default: return square_sums<__bf16>(group, partials, s);
+  Norm total = {partials, 0, max_norm, norm};
+  if (max_norm > 0.0) {
+    for (int i = 0; i < n_groups; ++i) {
+      const jtvae_adamw_group_t* g = groups + i;
+      double* p = partials + total.n;
+      switch (g->dtype) {
+        case JTVAE_F32: JT_CHECK(square_sums<float>(g, p, s)); break;
+        case JTVAE_F16: JT_CHECK(square_sums<_Float16>(g, p, s)); break;
+        default: JT_CHECK(square_sums<__bf16>(g, p, s));
+      }
+      total.n += g->n_chunks;
+    }
   }
-}
-
-int jtvae_grad_norm(const double* partials, int64_t n_partials, double max_norm, float* norm, void* stream) {
-  if (n_partials < 0) return JTVAE_E_SHAPE;
-  if (!norm || (n_partials && !partials)) return JTVAE_E_NULL;
-  if (!(max_norm > 0.0)) return JTVAE_E_RANGE;
-  hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(kNormBlock), 0, (hipStream_t)stream, partials, (long)n_partials,
-                     max_norm, norm);
-  return launch_status();
-}
-
-int jtvae_adamw_step(const jtvae_adamw_group_t* group, const float* grad_scale, void* stream) {
-  JT_CHECK(check_group(group));
-  const jtvae_adamw_group_t& g = *group;
-  if (!(g.beta1 >= 0.0 && g.beta1 < 1.0 && g.beta2 >= 0.0 && g.beta2 < 1.0 && g.eps >= 0.0)) return JTVAE_E_RANGE;
-  if (g.n_tensors == 0 || g.n_chunks == 0) return 0;
-  if (!g.steps || !g.bias) return JTVAE_E_NULL;
-  hipStream_t s = (hipStream_t)stream;
-  for (int t0 = 0; t0 < g.n_tensors; t0 += JTVAE_ADAMW_MAX_TENSORS) {
-    Present p = {};
-    p.first = t0;
-    p.count = g.n_tensors - t0 < JTVAE_ADAMW_MAX_TENSORS ? g.n_tensors - t0 : JTVAE_ADAMW_MAX_TENSORS;
-    for (int i = 0; i < p.count; ++i)
-      if (g.grads[t0 + i]) p.bits[i >> 5] |= 1u << (i & 31);
-    hipLaunchKernelGGL(steps_kernel, dim3((p.count + kBlock - 1) / kBlock), dim3(kBlock), 0, s, g.steps,
-                       (float2*)g.bias, p, g.beta1, g.beta2);
-    JT_CHECK(launch_status());
+  bool norm_due = max_norm > 0.0;
+  for (int i = 0; i < n_groups; ++i) {
+    const jtvae_adamw_group_t& g = groups[i];
+    for (int t0 = 0; t0 < g.n_tensors; t0 += JTVAE_ADAMW_MAX_TENSORS) {
+      Present p = {};
+      p.first = t0;
+      p.count = g.n_tensors - t0 < JTVAE_ADAMW_MAX_TENSORS ? g.n_tensors - t0 : JTVAE_ADAMW_MAX_TENSORS;
+      for (int k = 0; k < p.count; ++k)
+        if (g.grads[t0 + k]) p.bits[k >> 5] |= 1u << (k & 31);
+      hipLaunchKernelGGL(prepare_kernel, dim3(norm_due ? 2 : 1), dim3(kPrepBlock), 0, s, g.steps, (float2*)g.bias, p,
+                         g.beta1, g.beta2, total);
+      JT_CHECK(launch_status());
+      norm_due = false;
+    }
   }
-  const Hyper h = {(float)g.lr,    (float)g.weight_decay,  (float)g.beta1, (float)(1.0 - g.beta1),
-                   (float)g.beta2, (float)(1.0 - g.beta2), (float)g.eps,   g.lr_device,
-                   grad_scale};
-  const bool master = g.dtype != JTVAE_F32 && g.use_master;
-  switch (g.dtype) {
-    case JTVAE_F32: return step<float, false>(group, h, s);
-    case JTVAE_F16: return master ? step<_Float16, true>(group, h, s) : step<_Float16, false>(group, h, s);
-    default: return master ? step<__bf16, true>(group, h, s) : step<__bf16, false>(group, h, s);
+  for (int i = 0; i < n_groups; ++i) {
+    const jtvae_adamw_group_t& g = groups[i];
+    const Hyper h = {(float)g.lr,    (float)g.weight_decay,  (float)g.beta1, (float)(1.0 - g.beta1),
+                     (float)g.beta2, (float)(1.0 - g.beta2), (float)g.eps,   g.lr_device,
+                     max_norm > 0.0 ? norm + 1 : nullptr};
+    const bool master = g.dtype != JTVAE_F32 && g.use_master;
+    int rc;
+    switch (g.dtype) {
+      case JTVAE_F32: rc = step<float, false>(&g, h, s); break;
+      case JTVAE_F16: rc = master ? step<_Float16, true>(&g, h, s) : step<_Float16, false>(&g, h, s); break;
+      default: rc = master ? step<__bf16, true>(&g, h, s) : step<__bf16, false>(&g, h, s);
+    }
+    if (rc) return rc;
   }
+  return 0;
 }
 
 }  // extern "C"

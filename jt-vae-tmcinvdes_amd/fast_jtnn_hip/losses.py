@@ -15,6 +15,8 @@ logits' type and layout.  Statistics are fp32, sums over a sequence fp64; no ato
 """
 from __future__ import annotations
 
+import contextlib
+import functools
 from typing import NamedTuple, Optional
 
 import numpy as np
@@ -22,6 +24,18 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _capi as K
+
+
+def _differentiable_once(backward):
+    """torch's ``once_differentiable``, entered only where a graph of the backward pass is being built: the backward
+    runs on autograd's own thread, where every Python call counts."""
+    recorded = once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def call(ctx, *grads):
+        return recorded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return call
 
 
 class PreferenceLoss(NamedTuple):
@@ -88,6 +102,8 @@ class SequencePlan:
         views = [self._store[at:at + max(a.size, 1)] for a, at in zip(parts, ends)]
         self.row_seq, self.seq_ptr, self.seq_rows = views[:3]
         self.pairs, self.pair_ptr, self.pair_list = views[3:] if self.n_pairs is not None else (None,) * 3
+        self.arg = K.Sequences(self.row_seq.data_ptr(), self.seq_ptr.data_ptr(), self.seq_rows.data_ptr(), n_seq,
+                               K.ptr(self.pairs), self.n_pairs or 0, K.ptr(self.pair_ptr), K.ptr(self.pair_list))
 
     def on_current_stream(self):
         """Tells the allocator when the tables are read on another stream than the one they were made on."""
@@ -143,7 +159,9 @@ def _check_vector(what, name, t, n):
 
 def _fp32(t):
     """A per-row or per-sequence input as the kernels read it (None stays None)."""
-    return None if t is None else t.detach().float().contiguous()
+    if t is None or (t.dtype is torch.float32 and t.is_contiguous()):
+        return t
+    return t.detach().float().contiguous()
 
 
 def _number(what, name, v, lo, hi=float("inf")):
@@ -153,72 +171,84 @@ def _number(what, name, v, lo, hi=float("inf")):
     return v
 
 
+_NOTHING = contextlib.nullcontext()
+
+
+def _guard(device):
+    return _NOTHING if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
 def _rows(logits):
-    """The logits as rows of unit column stride (a copy only where columns are strided or rows overlap)."""
-    x = logits.detach()
-    n, v = x.shape
-    if (v > 1 and x.stride(1) != 1) or (n > 1 and x.stride(0) < v):
-        x = x.contiguous()
-    return x
+    """The logits themselves, or a copy where columns are strided or rows overlap."""
+    (n, v), (s0, s1) = logits.shape, logits.stride()
+    if (s1 != 1 and v > 1) or (s0 < v and n > 1):
+        return logits.detach().contiguous()
+    return logits
 
 
 def _arg(x, labels):
-    """(jtvae_logits_t, tensors to keep alive until the launch is enqueued)."""
-    labels = labels.detach().contiguous()
+    """(jtvae_logits_t, the labels as it names them: kept alive until the last launch that reads them)."""
+    labels = labels.contiguous()
     n, v = x.shape
-    ld = max(x.stride(0), v) if n > 1 else v
-    return K.logits_arg(x.data_ptr(), ld, n, v, K.DTYPE_CODE[x.dtype], labels.data_ptr(),
-                        64 if labels.dtype == torch.int64 else 32), labels
+    return K.Logits(x.data_ptr(), K.DTYPE_CODE[x.dtype], x.stride(0) if n > 1 else v, n, v, labels.data_ptr(),
+                    64 if labels.dtype is torch.int64 else 32), labels
 
 
-def _like_rows(x):
+def _again(ctx, x, labels):
+    """The backward pass's jtvae_logits_t: the forward's, unless the saved tensors came back at another place."""
+    g, keep = ctx.arg
+    if x.data_ptr() != g.x or labels.data_ptr() != g.labels:
+        ctx.arg = g, keep = _arg(x, labels)
+    return g
+
+
+def _grad_rows(x):
     """(uninitialised gradient in the layout of ``x``, its leading dimension): the few padding columns of the package's
     row buffers are kept - the kernel writes them as zero - so that the products that follow take it without a copy."""
-    ld = _like_ld(x)
-    return torch.empty((x.shape[0], ld), dtype=x.dtype, device=x.device)[:, :x.shape[1]], ld
+    n, v = x.shape
+    ld = _grad_ld(x)
+    if ld == v:
+        return torch.empty((n, v), dtype=x.dtype, device=x.device), ld
+    return torch.empty((n, ld), dtype=x.dtype, device=x.device)[:, :v], ld
 
 
-def _like_ld(x):
+def _grad_ld(x):
     n, v = x.shape
     ld = x.stride(0) if n > 1 else v
     return ld if v <= ld < v + 64 else v
 
 
-def _logits_grad(x, labels, owner, stats, coef, upstream):
-    d, ld = _like_rows(x)
-    if coef.numel() == 0:  # no sequences, so no row counts: an address that is never read
-        coef = coef.new_zeros(1)
-    g, keep = _arg(x, labels)
-    K.label_log_probs_bwd(g, K.ptr(owner), stats.data_ptr(), coef.data_ptr(), K.ptr(upstream), d.data_ptr(), ld, ld)
-    return d
-
-
-def _stats(x, labels, owner, want32, want64):
-    n, dev = x.shape[0], x.device
-    stats = torch.empty((n, 2), dtype=torch.float32, device=dev)
-    lp32 = torch.empty((n,), dtype=torch.float32, device=dev) if want32 else None
-    lp64 = torch.empty((max(n, 1),), dtype=torch.float64, device=dev) if want64 else None
-    g, keep = _arg(x, labels)
-    K.label_log_probs(g, K.ptr(owner), stats.data_ptr(), K.ptr(lp32), K.ptr(lp64))
-    return stats, lp32, lp64
+def _scratch(device, *counts):
+    """One buffer of 64-bit words for the pieces of the given lengths; (buffer, address of every piece)."""
+    buf = torch.empty((sum(counts) + 1,), dtype=torch.float64, device=device)
+    at, out = buf.data_ptr(), []
+    for c in counts:
+        out.append(at)
+        at += 8 * c
+    return buf, out
 
 
 class _TokenLogProbs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, labels):
-        x = _rows(logits)
-        with torch.cuda.device(x.device):
-            stats, lp, _ = _stats(x, labels, None, True, False)
-        ctx.save_for_backward(x if x.data_ptr() != logits.data_ptr() else logits, labels, stats)
+        x, dev, n = _rows(logits), logits.device, logits.shape[0]
+        with _guard(dev):
+            lp = torch.empty((n,), dtype=torch.float32, device=dev)
+            ctx.ws, (stats,) = _scratch(dev, n)
+            ctx.arg = g, _ = _arg(x, labels)
+            K.label_log_probs(g, None, stats, lp.data_ptr(), None)
+        ctx.save_for_backward(x, labels)
         return lp
 
     @staticmethod
-    @once_differentiable
+    @_differentiable_once
     def backward(ctx, dlp):
-        logits, labels, stats = ctx.saved_tensors
-        with torch.cuda.device(logits.device):
-            coef = dlp.detach().float().contiguous()
-            return _logits_grad(logits.detach(), labels, None, stats, coef, None), None
+        x, labels = ctx.saved_tensors
+        with _guard(x.device):
+            coef = dlp.float().contiguous()
+            d, ld = _grad_rows(x)
+            K.label_log_probs_bwd(_again(ctx, x, labels), None, ctx.ws.data_ptr(), coef.data_ptr(), None, d.data_ptr(), ld, ld)
+        return d, None
 
 
 def token_log_probs(logits: torch.Tensor, labels: torch.Tensor) -> torch.Tensor:
@@ -231,24 +261,29 @@ def token_log_probs(logits: torch.Tensor, labels: torch.Tensor) -> torch.Tensor:
 class _SequenceLogProbs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, labels, plan):
-        x = _rows(logits)
-        with torch.cuda.device(x.device):
+        x, dev, n = _rows(logits), logits.device, logits.shape[0]
+        with _guard(dev):
             plan.on_current_stream()
-            stats, _, lp64 = _stats(x, labels, plan.row_seq, False, True)
-            sums = torch.empty((plan.n_seq,), dtype=torch.float32, device=x.device)
-            K.sequence_sums(lp64.data_ptr(), plan.seq_ptr.data_ptr(), plan.seq_rows.data_ptr(), plan.n_seq, None, None,
-                            sums.data_ptr(), n_rows=x.shape[0])
-        ctx.save_for_backward(x if x.data_ptr() != logits.data_ptr() else logits, labels, stats)
+            sums = torch.empty((plan.n_seq,), dtype=torch.float32, device=dev)
+            ctx.ws, (stats, ws) = _scratch(dev, n, n)
+            ctx.arg = g, _ = _arg(x, labels)
+            K.sequence_log_probs(g, plan.arg, stats, sums.data_ptr(), ws, 8 * n)
+        ctx.save_for_backward(x, labels)
         ctx.plan = plan
         return sums
 
     @staticmethod
-    @once_differentiable
+    @_differentiable_once
     def backward(ctx, dsums):
-        logits, labels, stats = ctx.saved_tensors
-        with torch.cuda.device(logits.device):
-            coef = dsums.detach().float().contiguous()
-            return _logits_grad(logits.detach(), labels, ctx.plan.row_seq, stats, coef, None), None, None
+        x, labels = ctx.saved_tensors
+        with _guard(x.device):
+            coef = dsums.float().contiguous()
+            d, ld = _grad_rows(x)
+            g, keep = _arg(x, labels)
+            # without sequences no row counts and the coefficients are never read: any address will do
+            K.label_log_probs_bwd(g, ctx.plan.arg.row_seq, ctx.ws.data_ptr(), coef.data_ptr() or ctx.ws.data_ptr(), None,
+                                  d.data_ptr(), ld, ld)
+        return d, None, None
 
 
 def sequence_log_probs(logits: torch.Tensor, labels: torch.Tensor, plan: SequencePlan) -> torch.Tensor:
@@ -263,40 +298,45 @@ def sequence_log_probs(logits: torch.Tensor, labels: torch.Tensor, plan: Sequenc
 class _PreferenceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, other, labels, plan, ref, beta, smoothing, scale):
-        x, dev, S, P = _rows(logits), logits.device, plan.n_seq, plan.n_pairs
-        with torch.cuda.device(dev):
+        x, dev, n, S, P = _rows(logits), logits.device, logits.shape[0], plan.n_seq, plan.n_pairs
+        with _guard(dev):
             plan.on_current_stream()
             oth, ref = _fp32(other), _fp32(ref)
-            stats, _, lp64 = _stats(x, labels, plan.row_seq, False, True)
-            sums64 = torch.empty((S,), dtype=torch.float64, device=dev)
-            dmargin = torch.empty((P,), dtype=torch.float64, device=dev)
-            sums, coef = (torch.empty((S,), dtype=torch.float32, device=dev) for _ in range(2))
+            sums = torch.empty((S,), dtype=torch.float32, device=dev)
             margins = torch.empty((P,), dtype=torch.float32, device=dev)
             loss = torch.empty((), dtype=torch.float32, device=dev)
-            K.sequence_sums(lp64.data_ptr(), plan.seq_ptr.data_ptr(), plan.seq_rows.data_ptr(), S, K.ptr(oth),
-                            sums64.data_ptr(), sums.data_ptr(), n_rows=x.shape[0])
-            K.preference_pairs(sums64.data_ptr(), ref.data_ptr(), plan.pairs.data_ptr(), P, plan.pair_ptr.data_ptr(),
-                               plan.pair_list.data_ptr(), S, beta, smoothing, scale, loss.data_ptr(),
-                               margins.data_ptr(), dmargin.data_ptr(), coef.data_ptr())
-        ctx.save_for_backward(x if x.data_ptr() != logits.data_ptr() else logits, labels, stats, coef)
+            ctx.ws, (stats, coef, ws) = _scratch(dev, n, (S + 1) // 2, n + S + P)
+            ctx.arg = g, _ = _arg(x, labels)
+            K.preference_loss(g, plan.arg, K.Preference(ref.data_ptr(), K.ptr(oth), beta, smoothing, scale), stats,
+                              sums.data_ptr(), margins.data_ptr(), coef, loss.data_ptr(), ws, 8 * (n + S + P))
+        ctx.save_for_backward(x, labels)
         ctx.plan, ctx.other_dtype = plan, None if other is None else other.dtype
         ctx.mark_non_differentiable(sums, margins)
         ctx.set_materialize_grads(False)
         return loss, sums, margins
 
     @staticmethod
-    @once_differentiable
+    @_differentiable_once
     def backward(ctx, dloss, *_):
         if dloss is None:
             return (None,) * 8
-        logits, labels, stats, coef = ctx.saved_tensors
-        d = dother = None
-        with torch.cuda.device(logits.device):
-            up = dloss.detach().float().contiguous()
-            if ctx.needs_input_grad[0]:
-                d = _logits_grad(logits.detach(), labels, ctx.plan.row_seq, stats, coef, up)
+        x, labels = ctx.saved_tensors
+        plan, d, dother = ctx.plan, None, None
+        stats = ctx.ws.data_ptr()
+        coef = stats + 8 * x.shape[0]
+        with _guard(x.device):
+            up = dloss.float()
             if ctx.needs_input_grad[1]:
-                dother = (coef * up).to(ctx.other_dtype)
+                dother = torch.empty((plan.n_seq,), dtype=torch.float32, device=x.device)
+            if ctx.needs_input_grad[0]:
+                d, ld = _grad_rows(x)
+                K.label_log_probs_bwd(_again(ctx, x, labels), plan.arg.row_seq, stats, coef, up.data_ptr(), d.data_ptr(), ld, ld,
+                                      scaled=K.ptr(dother), n_scaled=0 if dother is None else plan.n_seq)
+            elif dother is not None:
+                at = 2 * x.shape[0]
+                torch.mul(ctx.ws.view(torch.float32)[at:at + plan.n_seq], up, out=dother)
+            if dother is not None and ctx.other_dtype is not torch.float32:
+                dother = dother.to(ctx.other_dtype)
         return d, dother, None, None, None, None, None, None
 
 
@@ -328,42 +368,42 @@ class _PolicyLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, labels, old, adv, ref, weights, lo, hi, kl_coef, scale):
         x, dev, n = _rows(logits), logits.device, logits.shape[0]
-        with torch.cuda.device(dev):
+        with _guard(dev):
             old, adv, ref, weights = (_fp32(t) for t in (old, adv, ref, weights))
-            stats = torch.empty((n, 2), dtype=torch.float32, device=dev)
-            lp, coef = (torch.empty((n,), dtype=torch.float32, device=dev) for _ in range(2))
+            lp = torch.empty((n,), dtype=torch.float32, device=dev)
             loss, kl, clipped = (torch.empty((), dtype=torch.float32, device=dev) for _ in range(3))
             nbytes = K.policy_loss_workspace_bytes(n)
-            ws = torch.empty((max(nbytes, 16),), dtype=torch.uint8, device=dev)
-            g, keep = _arg(x, labels)
-            policy = K.Policy(old.data_ptr(), adv.data_ptr(), K.ptr(ref), K.ptr(weights), lo, hi, kl_coef, scale)
+            ctx.ws, (stats, coef, ws) = _scratch(dev, n, (n + 1) // 2, nbytes // 8)
             # a row's coefficient depends on that row alone: its gradient is made while the row is in registers
-            d, ld = _like_rows(x) if ctx.needs_input_grad[0] else (None, 0)
-            K.policy_loss(g, policy, stats.data_ptr(), lp.data_ptr(), coef.data_ptr(), loss.data_ptr(), kl.data_ptr(),
-                          clipped.data_ptr(), K.ptr(d), ld, ld, ws.data_ptr(), nbytes)
-        ctx.save_for_backward(x if x.data_ptr() != logits.data_ptr() else logits, labels, stats, coef)
+            d, ld = _grad_rows(x) if ctx.needs_input_grad[0] else (None, 0)
+            ctx.arg = g, _ = _arg(x, labels)
+            policy = K.Policy(old.data_ptr(), adv.data_ptr(), K.ptr(ref), K.ptr(weights), lo, hi, kl_coef, scale)
+            K.policy_loss(g, policy, stats, lp.data_ptr(), coef, loss.data_ptr(), kl.data_ptr(), clipped.data_ptr(),
+                          K.ptr(d), ld, ld, ws, nbytes)
+        ctx.save_for_backward(x, labels)
         ctx.gradient = d
         ctx.mark_non_differentiable(lp, kl, clipped)
         ctx.set_materialize_grads(False)
         return loss, lp, kl, clipped
 
     @staticmethod
-    @once_differentiable
+    @_differentiable_once
     def backward(ctx, dloss, *_):
         if dloss is None:
             return (None,) * 10
-        logits, labels, stats, coef = ctx.saved_tensors
+        x, labels = ctx.saved_tensors
         d, ctx.gradient = ctx.gradient, None
-        with torch.cuda.device(logits.device):
-            up = dloss.detach().float().contiguous()
-            x = logits.detach()
-            if d is None:  # a second pass through the graph: the first one's gradient has been given away
-                d = _logits_grad(x, labels, None, stats, coef, up)
-            else:  # stands as it is where the upstream factor is 1, which only the device knows
-                g, keep = _arg(x, labels)
-                ld = _like_ld(x)
-                K.label_log_probs_bwd(g, None, stats.data_ptr(), coef.data_ptr(), up.data_ptr(), d.data_ptr(), ld, ld,
-                                      unless_one=True)
+        fresh = d is not None  # else a second pass through the graph: the first one's gradient has been given away
+        with _guard(x.device):
+            up = dloss.float()
+            if fresh:
+                ld = _grad_ld(x)
+            else:
+                d, ld = _grad_rows(x)
+            stats = ctx.ws.data_ptr()
+            # a fresh gradient stands as it is where the upstream factor is 1, which only the device knows
+            K.label_log_probs_bwd(_again(ctx, x, labels), None, stats, stats + 8 * x.shape[0], up.data_ptr(), d.data_ptr(), ld, ld,
+                                  unless_one=int(fresh))
         return (d,) + (None,) * 9
 
 

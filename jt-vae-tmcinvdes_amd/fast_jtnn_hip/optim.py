@@ -102,20 +102,18 @@ class _Group:
 
     def gather_grads(self):
         """Fills the address list; (parameters with a gradient, tensors to keep alive until the launches)."""
-        have, keep, grads = [], [], self.grads
-        for i, p in enumerate(self.params):
+        keep, at = [], []
+        for p in self.params:
             g = p.grad
             if g is None:
-                grads[i] = None
+                at.append(None)
                 continue
-            if g.layout is not torch.strided:
-                raise RuntimeError("AdamW does not take sparse gradients")
             if not g.is_contiguous():
                 g = g.contiguous()
                 keep.append(g)
-            grads[i] = g.data_ptr()
-            have.append(p)
-        return have, keep
+            at.append(g.data_ptr())
+        self.grads[:] = at
+        return (self.params if None not in at else [p for p, a in zip(self.params, at) if a is not None]), keep
 
     def args(self, hyper):
         lr = hyper["lr"]
@@ -227,40 +225,30 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        max_norm = 0.0 if self.max_norm is None else float(self._check_norm(self.max_norm))
         with torch.cuda.device(self._bound[0].device):
-            work, keep, changed = [], [], []
+            work, keep, args, changed = [], [], [], []
             for g, hyper in zip(self._bound, self.param_groups):
                 self._check_hyper(hyper)
                 g.bind()
                 have, k = g.gather_grads()
-                keep += k
                 if have:
+                    keep += k
                     changed += have
-                    work.append((g, g.args(hyper)))
-            scale = None
-            if self.max_norm is not None and work:
-                self._clip_factor(work)
-                scale = self._norm.data_ptr() + 4
-            for g, args in work:
-                K.adamw_step(args, scale, n_elems=g.n_elems)
+                    work.append(g)
+                    args.append(g.args(hyper))
+            if not work:
+                return loss
+            partials = None
+            if max_norm:
+                partials = work[0].partials if len(work) == 1 else \
+                    torch.empty(sum(g.n_chunks for g in work), dtype=torch.float64, device=self._norm.device)
+            K.adamw_step((K.AdamwGroup * len(args))(*args), len(args), max_norm, K.ptr(partials),
+                         self._norm.data_ptr(), n_elems=[g.n_elems for g in work])
             # the kernels wrote through raw addresses: weights packed for the products, and autograd's check of saved
             # tensors, go by the version counter
-            if changed:
-                torch.autograd.graph.increment_version(changed)
+            torch.autograd.graph.increment_version(changed)
         return loss
-
-    def _clip_factor(self, work):
-        max_norm = float(self._check_norm(self.max_norm))
-        if len(work) == 1:
-            partials = work[0][0].partials
-        else:
-            n = sum(g.n_chunks for g, _ in work)
-            partials = torch.empty(n, dtype=torch.float64, device=self._norm.device)
-        at = 0
-        for g, args in work:
-            K.grad_square_sums(args, partials.data_ptr() + 8 * at, n_elems=g.n_elems)
-            at += g.n_chunks
-        K.grad_norm(partials.data_ptr(), at, max_norm, self._norm.data_ptr())
 
     @torch.no_grad()
     def load_state_dict(self, state_dict):

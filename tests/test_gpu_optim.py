@@ -305,6 +305,10 @@ def test_works_with_schedulers_strided_gradients_and_closures():
     p.grad = torch.ones(1, 1, device="cuda").expand(64, 32)
     opt.step()
     assert torch.allclose(p, torch.full_like(p, 0.25), atol=1e-6)
+    q = torch.nn.Parameter(torch.ones(4, 2, device="cuda"))
+    q.grad = torch.sparse_coo_tensor([[0], [1]], [1.0], (4, 2), device="cuda")
+    with pytest.raises(RuntimeError):  # sparse gradients are not taken
+        AdamW([q]).step()
     opt.zero_grad()
     before = p.detach().clone()
     opt.step()  # no gradients: nothing happens

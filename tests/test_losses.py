@@ -97,34 +97,53 @@ def test_adamw_arguments_refused():
 
 def test_c_entry_points_refuse_before_launch():
     lib = K.lib
-    ok = K.logits_arg(256, 8, 4, 7, K.F32, 256, 64)
+    ok = K.Logits(256, K.F32, 8, 4, 7, 256, 64)
 
     def lp(g, stats=256):
         return lib.jtvae_label_log_probs(ctypes.byref(g), None, stats, 256, None, None)
 
     assert lib.jtvae_label_log_probs(None, None, 256, 256, None, None) == K.E_NULL
     assert lp(ok, None) == K.E_NULL
-    assert lp(K.logits_arg(256, 6, 4, 7, K.F32, 256, 64)) == K.E_SHAPE  # ld < n_cols
-    assert lp(K.logits_arg(256, 8, -1, 7, K.F32, 256, 64)) == K.E_SHAPE
-    assert lp(K.logits_arg(256, 8, 4, 0, K.F32, 256, 64)) == K.E_SHAPE
-    assert lp(K.logits_arg(256, 8, 4, 7, 3, 256, 64)) == K.E_RANGE
-    assert lp(K.logits_arg(256, 8, 4, 7, K.F32, 256, 16)) == K.E_RANGE
-    assert lp(K.logits_arg(None, 8, 4, 7, K.F32, 256, 64)) == K.E_NULL
-    assert lp(K.logits_arg(258, 8, 4, 7, K.F32, 256, 64)) == K.E_ALIGN
-    assert lp(K.logits_arg(258, 8, 4, 7, K.BF16, 260, 64)) == K.E_ALIGN
-    assert lp(K.logits_arg(None, 8, 0, 7, K.F32, None, 64)) == 0  # no rows: nothing to do
+    assert lp(K.Logits(256, K.F32, 6, 4, 7, 256, 64)) == K.E_SHAPE  # ld < n_cols
+    assert lp(K.Logits(256, K.F32, 8, -1, 7, 256, 64)) == K.E_SHAPE
+    assert lp(K.Logits(256, K.F32, 8, 4, 0, 256, 64)) == K.E_SHAPE
+    assert lp(K.Logits(256, 3, 8, 4, 7, 256, 64)) == K.E_RANGE
+    assert lp(K.Logits(256, K.F32, 8, 4, 7, 256, 16)) == K.E_RANGE
+    assert lp(K.Logits(None, K.F32, 8, 4, 7, 256, 64)) == K.E_NULL
+    assert lp(K.Logits(258, K.F32, 8, 4, 7, 256, 64)) == K.E_ALIGN
+    assert lp(K.Logits(258, K.BF16, 8, 4, 7, 260, 64)) == K.E_ALIGN
+    assert lp(K.Logits(None, K.F32, 8, 0, 7, None, 64)) == 0  # no rows: nothing to do
     bwd = lib.jtvae_label_log_probs_bwd
-    assert bwd(ctypes.byref(ok), None, 256, 256, None, 0, 256, 7, 8, None) == K.E_SHAPE  # width > ld_dx
-    assert bwd(ctypes.byref(ok), None, 256, 256, None, 0, 256, 8, 6, None) == K.E_SHAPE  # width < n_cols
-    assert bwd(ctypes.byref(ok), None, 256, 256, None, 0, 257, 8, 8, None) == K.E_ALIGN
-    assert bwd(ctypes.byref(ok), None, None, 256, None, 0, 256, 8, 8, None) == K.E_NULL
-    assert bwd(ctypes.byref(ok), None, 256, 256, None, 1, 256, 8, 8, None) == K.E_NULL  # unless_one without upstream
-    assert lib.jtvae_sequence_sums(None, None, None, 0, None, None, None, None) == 0
-    assert lib.jtvae_sequence_sums(None, 256, 256, 2, None, None, 256, None) == K.E_NULL
-    assert lib.jtvae_sequence_sums(256, 256, 256, -2, None, None, 256, None) == K.E_SHAPE
-    pairs = lambda n=1, e=0.0, loss=256: lib.jtvae_preference_pairs(  # noqa: E731
-        256, 256, 256, n, 256, 256, 2, 0.1, e, 1.0, loss, 256, 256, None, None)
-    assert pairs() == K.E_NULL and pairs(n=-1) == K.E_SHAPE and pairs(loss=None) == K.E_NULL
+    assert bwd(ctypes.byref(ok), None, 256, 256, None, 0, 256, 7, 8, None, 0, None) == K.E_SHAPE  # width > ld_dx
+    assert bwd(ctypes.byref(ok), None, 256, 256, None, 0, 256, 8, 6, None, 0, None) == K.E_SHAPE  # width < n_cols
+    assert bwd(ctypes.byref(ok), None, 256, 256, None, 0, 257, 8, 8, None, 0, None) == K.E_ALIGN
+    assert bwd(ctypes.byref(ok), None, None, 256, None, 0, 256, 8, 8, None, 0, None) == K.E_NULL
+    assert bwd(ctypes.byref(ok), None, 256, 256, None, 1, 256, 8, 8, None, 0, None) == K.E_NULL  # unless_one without upstream
+    assert bwd(ctypes.byref(ok), None, 256, 256, None, 0, 256, 8, 8, 256, -1, None) == K.E_SHAPE
+    assert bwd(ctypes.byref(ok), None, 256, 256, None, 0, 256, 8, 8, None, 2, None) == K.E_NULL
+    seqs = K.Sequences(256, 256, 256, 2, 256, 1, 256, 256)
+    pref = K.Preference(256, None, 0.1, 0.0, 1.0)
+    none = K.Logits(None, K.F32, 8, 0, 7, None, 64)
+
+    def sums(q=seqs, ws=32, sums=256, stats=256):
+        return lib.jtvae_sequence_log_probs(ctypes.byref(ok), ctypes.byref(q), stats, sums, 256, ws, None)
+
+    assert K.lib.jtvae_sequence_log_probs_workspace_bytes(4) == 32
+    assert sums(ws=31) == K.E_WORKSPACE and sums(sums=None) == K.E_NULL and sums(stats=None) == K.E_NULL
+    assert sums(q=K.Sequences(None, 256, 256, 2, None, 0, None, None)) == K.E_NULL
+    assert sums(q=K.Sequences(256, 256, 256, -1, None, 0, None, None)) == K.E_SHAPE
+    assert lib.jtvae_sequence_log_probs(ctypes.byref(none), ctypes.byref(K.Sequences()), None, None, None, 0, None) == 0
+
+    def pairs(q=seqs, p=pref, ws=56, loss=256, coef=256):
+        return lib.jtvae_preference_loss(ctypes.byref(ok), ctypes.byref(q), ctypes.byref(p), 256, 256, 256, coef, loss, 256,
+                                         ws, None)
+
+    assert K.lib.jtvae_preference_loss_workspace_bytes(4, 2, 1) == 56
+    assert pairs(ws=55) == K.E_WORKSPACE and pairs(loss=None) == K.E_NULL and pairs(coef=None) == K.E_NULL
+    assert pairs(p=K.Preference(None, None, 0.1, 0.0, 1.0)) == K.E_NULL
+    assert pairs(p=K.Preference(256, None, 0.1, 1.5, 1.0)) == K.E_RANGE
+    assert pairs(q=K.Sequences(256, 256, 256, 2, None, 1, 256, 256)) == K.E_NULL
+    assert pairs(q=K.Sequences(256, 256, 256, 2, 256, -1, 256, 256)) == K.E_SHAPE
     pol = K.Policy(256, 256, None, None, 0.2, 0.2, 0.0, 1.0)
     need = K.policy_loss_workspace_bytes(4)
     assert need > 0 and K.policy_loss_workspace_bytes(0) == 0
@@ -135,9 +154,6 @@ def test_c_entry_points_refuse_before_launch():
     assert policy(ws=need - 1) == K.E_WORKSPACE and policy(stats=None) == K.E_NULL and policy(loss=None) == K.E_NULL
     assert policy(p=K.Policy(None, 256, None, None, 0.2, 0.2, 0.0, 1.0)) == K.E_NULL
     assert policy(p=K.Policy(256, 256, None, None, 1.2, 0.2, 0.0, 1.0)) == K.E_RANGE
-    assert lib.jtvae_grad_norm(None, 3, 1.0, 256, None) == K.E_NULL
-    assert lib.jtvae_grad_norm(256, 3, 0.0, 256, None) == K.E_RANGE
-    assert lib.jtvae_grad_norm(256, -3, 1.0, 256, None) == K.E_SHAPE
     ptr = (ctypes.c_int64 * 2)(0, 1)
     grads = (ctypes.c_void_p * 1)(None)
 
@@ -152,7 +168,10 @@ def test_c_entry_points_refuse_before_launch():
                      (dict(dtype=7), K.E_RANGE), (dict(state_bits=16), K.E_RANGE), (dict(n_tensors=-1), K.E_SHAPE),
                      (dict(n_chunks=2), K.E_SHAPE), (dict(beta1=1.0), K.E_RANGE), (dict(eps=-1.0), K.E_RANGE),
                      (dict(steps=None), K.E_NULL)):
-        assert lib.jtvae_adamw_step(ctypes.byref(group(**kw)), None, None) == code, kw
-    assert lib.jtvae_adamw_step(None, None, None) == K.E_NULL
-    assert lib.jtvae_grad_square_sums(ctypes.byref(group()), None, None) == K.E_NULL
-    assert lib.jtvae_grad_square_sums(ctypes.byref(group(dtype=7)), 256, None) == K.E_RANGE
+        assert lib.jtvae_adamw_step(ctypes.byref(group(**kw)), 1, 0.0, None, None, None) == code, kw
+    step = lambda n, norm, partials=256, out=256: lib.jtvae_adamw_step(  # noqa: E731
+        ctypes.byref(group()), n, norm, partials, out, None)
+    assert lib.jtvae_adamw_step(None, 1, 0.0, None, None, None) == K.E_NULL
+    assert lib.jtvae_adamw_step(None, 0, 0.0, None, None, None) == 0
+    assert step(-1, 0.0) == K.E_SHAPE and step(1, -1.0) == K.E_RANGE and step(1, float("nan")) == K.E_RANGE
+    assert step(1, 1.0, partials=None) == K.E_NULL and step(1, 1.0, out=None) == K.E_NULL
