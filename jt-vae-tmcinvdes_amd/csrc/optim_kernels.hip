@@ -250,6 +250,8 @@ struct Piece {
       r[k] = root(v[k]);
       // reciprocal on the hardware unit (1 ulp): the update is off by 2^-22 of itself, below half an ulp of w
       w[k] = w[k] * s.keep - s.rate * (m[k] * __builtin_amdgcn_rcpf(r[k] * s.bias2 + s.eps));
+      // a 16-bit parameter is the 32-bit value rounded: the compiler must not round the sum to 16 bits by itself
+      if constexpr (sizeof(T) == 2) asm("" : "+v"(w[k]));
     }
     if constexpr (MASTER) store<WHOLE, N>(t.master, at, t.n, w);
     store<WHOLE, N>((T*)t.param, at, t.n, w);
