@@ -63,8 +63,10 @@ __device__ __forceinline__ double label_log_prob(const T* row, long label, int n
   return ((double)(float)row[label] - (double)st.m) - log((double)st.s);
 }
 
-// Sixteen bytes of a row.  Rows start wherever the element type may stand (odd vocabularies, sliced views): the
-// hardware takes a 16-byte access at any address, and a wave's 1 KiB then touches nine cache lines instead of eight.
+// Sixteen bytes of a row.  Rows start wherever the element type may stand (odd vocabularies, sliced views): the few
+// elements before the first 16-byte boundary and after the last are taken one by one (see Shape), the vectors between
+// are aligned.  Reading vectors from the row's start instead, which the hardware allows, costs 12 % on 1500 x 50021
+// fp16.  The gradient's rows mostly stand like the logits'; where they do not, its stores cross the boundaries.
 typedef unsigned Word4 __attribute__((ext_vector_type(4)));
 typedef unsigned Word4At2 __attribute__((ext_vector_type(4), aligned(2)));
 typedef unsigned Word4At4 __attribute__((ext_vector_type(4), aligned(4)));
@@ -72,8 +74,9 @@ typedef unsigned Word4At4 __attribute__((ext_vector_type(4), aligned(4)));
 template <typename T>
 struct Vec {
   static constexpr int E = 16 / sizeof(T);
-  static __device__ __forceinline__ Word4 load(const T* p) { return *(const Word4At2*)p; }
-  static __device__ __forceinline__ void store(T* p, Word4 w) { *(Word4At2*)p = w; }
+  static __device__ __forceinline__ Word4 load(const T* p) { return *(const Word4*)p; }
+  static __device__ __forceinline__ Word4 load_once(const T* p) { return __builtin_nontemporal_load((const Word4*)p); }
+  static __device__ __forceinline__ void store(T* p, Word4 w) { __builtin_nontemporal_store(w, (Word4At2*)p); }
   static __device__ __forceinline__ void unpack(Word4 w, float v[E]) {
     T h[E];
     __builtin_memcpy(h, &w, 16);
@@ -92,13 +95,33 @@ struct Vec {
 template <>
 struct Vec<float> {
   static constexpr int E = 4;
-  static __device__ __forceinline__ Word4 load(const float* p) { return *(const Word4At4*)p; }
-  static __device__ __forceinline__ void store(float* p, Word4 w) { *(Word4At4*)p = w; }
+  static __device__ __forceinline__ Word4 load(const float* p) { return *(const Word4*)p; }
+  static __device__ __forceinline__ Word4 load_once(const float* p) {
+    return __builtin_nontemporal_load((const Word4*)p);
+  }
+  static __device__ __forceinline__ void store(float* p, Word4 w) { __builtin_nontemporal_store(w, (Word4At4*)p); }
   static __device__ __forceinline__ void unpack(Word4 w, float v[4]) { __builtin_memcpy(v, &w, 16); }
   static __device__ __forceinline__ Word4 pack(const float v[4]) {
     Word4 w;
     __builtin_memcpy(&w, v, 16);
     return w;
+  }
+};
+
+// How a row is cut: `head` elements, n_vec vectors, `tail` elements.  Lane t takes the single element extra(t), if any.
+template <typename T>
+struct Shape {
+  int head, n_vec, n_cols;
+  __device__ __forceinline__ Shape(const T* row, int cols) {
+    constexpr int E = Vec<T>::E;
+    head = (int)((16 - ((uintptr_t)row & 15)) & 15) / (int)sizeof(T);
+    head = head < cols ? head : cols;
+    n_vec = (cols - head) / E;
+    n_cols = cols;
+  }
+  __device__ __forceinline__ int col(int i) const { return head + i * Vec<T>::E; }
+  __device__ __forceinline__ int extra(int t) const {  // >= n_cols: none
+    return t < head ? t : n_vec * Vec<T>::E + t;
   }
 };
 
@@ -188,13 +211,14 @@ __global__ __launch_bounds__(BLOCK) void stats_kernel(RowsIn<T> in) {
     return;
   }
   const T* r = in.x + (long)row * in.ld;
-  const int n_vec = in.n_cols / E;
+  const Shape<T> shape(r, in.n_cols);
+  const int n_vec = shape.n_vec;
   RowStat st = {-INFINITY, 0.f};
   int i = threadIdx.x;
   for (; i + (U - 1) * BLOCK < n_vec; i += U * BLOCK) {
     Word4 w[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) w[u] = Vec<T>::load(r + (long)(i + u * BLOCK) * E);
+    for (int u = 0; u < U; ++u) w[u] = Vec<T>::load(r + shape.col(i + u * BLOCK));
     float v[U * E];
 #pragma unroll
     for (int u = 0; u < U; ++u) Vec<T>::unpack(w[u], v + u * E);
@@ -202,10 +226,10 @@ __global__ __launch_bounds__(BLOCK) void stats_kernel(RowsIn<T> in) {
   }
   for (; i < n_vec; i += BLOCK) {
     float v[E];
-    Vec<T>::unpack(Vec<T>::load(r + (long)i * E), v);
+    Vec<T>::unpack(Vec<T>::load(r + shape.col(i)), v);
     take<E>(st, v);
   }
-  const int c = n_vec * E + threadIdx.x;
+  const int c = shape.extra(threadIdx.x);
   if (c < in.n_cols) {
     const float v = (float)r[c];
     take<1>(st, &v);
@@ -244,7 +268,7 @@ enum { kStats = 0, kPolicy = 1 };
 // row depending on nothing else, its gradient in the same pass.  A block of RT * R threads owns R rows; the 64-bit
 // arithmetic of a row's end is done by one lane per row, side by side.
 template <typename T, int RT, int R, int NV, int MODE>
-__global__ __launch_bounds__(RT* R, NV > 8 ? 4 : 8) void rows_kernel(RowsIn<T> in, PolicyIn policy, float* __restrict__ coef,
+__global__ __launch_bounds__(RT* R, NV > 8 ? 4 : RT == 64 && NV == 8 ? 6 : 8) void rows_kernel(RowsIn<T> in, PolicyIn policy, float* __restrict__ coef,
                                                      double* __restrict__ terms, GradOut<T> out) {
   constexpr int E = Vec<T>::E, W = RT / 64;
   __shared__ RowStat part[R * W];
@@ -255,23 +279,37 @@ __global__ __launch_bounds__(RT* R, NV > 8 ? 4 : 8) void rows_kernel(RowsIn<T> i
   const long label = there ? in.labels[row] : -1;
   const bool counted = there && counts(in, row, label);
   const T* x = in.x + (long)row * in.ld;
-  const int n_vec = in.n_cols / E, c_tail = n_vec * E + t;
+  const Shape<T> shape(x, in.n_cols);
+  const int n_vec = shape.n_vec, c_one = shape.extra(t);
   Word4 w[NV];
-  float tail = -INFINITY;
+  float one = -INFINITY;
   RowStat st = {-INFINITY, 0.f};
   if (counted) {
 #pragma unroll
     for (int u = 0; u < NV; ++u)
-      if (t + u * RT < n_vec) w[u] = Vec<T>::load(x + (long)(t + u * RT) * E);
-    if (c_tail < in.n_cols) tail = (float)x[c_tail];
+      if (t + u * RT < n_vec) w[u] = Vec<T>::load(x + shape.col(t + u * RT));
+    if (c_one < in.n_cols) one = (float)x[c_one];
+    // the maximum of all that a lane holds first, so that every value takes one exponential
+    st.m = one;
 #pragma unroll
     for (int u = 0; u < NV; ++u)
       if (t + u * RT < n_vec) {
         float v[E];
         Vec<T>::unpack(w[u], v);
-        take<E>(st, v);
+#pragma unroll
+        for (int e = 0; e < E; ++e) st.m = fmaxf(st.m, v[e]);
       }
-    take<1>(st, &tail);
+    const float ref = finite_or_zero(st.m);
+    st.s = exp_nat(one - ref);
+#pragma unroll
+    for (int u = 0; u < NV; ++u)
+      if (t + u * RT < n_vec) {
+        float v[E];
+        asm("" : "+v"(w[u]));  // unpacked again, not kept unpacked: that takes twice the registers
+        Vec<T>::unpack(w[u], v);
+#pragma unroll
+        for (int e = 0; e < E; ++e) st.s += exp_nat(v[e] - ref);
+      }
     st = wave_join(st);
     if ((t & 63) == 0) part[threadIdx.x >> 6] = st;
   }
@@ -312,20 +350,20 @@ __global__ __launch_bounds__(RT* R, NV > 8 ? 4 : 8) void rows_kernel(RowsIn<T> i
       float v[E];
       if (counted) {
         Vec<T>::unpack(w[u], v);
-        softmax_grad<E>(v, (long)i * E, label, m, ks, k);
+        softmax_grad<E>(v, shape.col(i), label, m, ks, k);
       } else {
 #pragma unroll
         for (int e = 0; e < E; ++e) v[e] = 0.f;
       }
-      Vec<T>::store(d + (long)i * E, Vec<T>::pack(v));
+      Vec<T>::store(d + shape.col(i), Vec<T>::pack(v));
     }
-    if (c_tail < in.n_cols) {
+    if (c_one < in.n_cols) {
       float v = 0.f;
       if (counted) {
-        v = tail;
-        softmax_grad<1>(&v, c_tail, label, m, ks, k);
+        v = one;
+        softmax_grad<1>(&v, c_one, label, m, ks, k);
       }
-      d[c_tail] = (T)v;
+      d[c_one] = (T)v;
     }
     for (long c = in.n_cols + t; c < out.width; c += RT) d[c] = (T)0.f;
   }
@@ -334,7 +372,7 @@ __global__ __launch_bounds__(RT* R, NV > 8 ? 4 : 8) void rows_kernel(RowsIn<T> i
 // dx[row, j] = c ([j = label] - exp(x_j - m) / s), c = coef[owner or row] * upstream, from saved statistics.  Rows are
 // cut into tiles of RT lanes x NV vectors; a block of 256 threads owns 256 / RT tiles.  With unless_one the gradient
 // for an upstream factor of one is in place already and nothing is done where the factor is one.
-template <typename T, int RT, int NV>
+template <typename T, int RT, int NV, bool ONCE>
 __global__ __launch_bounds__(JTVAE_BLOCK) void grad_kernel(RowsIn<T> in, const float* __restrict__ coef,
                                                            const float* __restrict__ upstream, int unless_one,
                                                            int tiles, GradOut<T> out, float* __restrict__ scaled,
@@ -344,48 +382,56 @@ __global__ __launch_bounds__(JTVAE_BLOCK) void grad_kernel(RowsIn<T> in, const f
   for (long i = (long)blockIdx.x * JTVAE_BLOCK + threadIdx.x; i < n_scaled; i += (long)gridDim.x * JTVAE_BLOCK)
     scaled[i] = coef[i] * up;
   if (unless_one && up == 1.f) return;
-  const long id = (long)blockIdx.x * (JTVAE_BLOCK / RT) + threadIdx.x / RT;
-  const int row = (int)(id / tiles), tile = (int)(id - (long)row * tiles), t = threadIdx.x % RT;
-  if (row >= in.n_rows) return;
-  const long label = in.labels[row];
-  const int own = in.owner ? in.owner[row] : row;
-  const bool counted = label >= 0 && own >= 0;
-  const T* x = in.x + (long)row * in.ld;
-  T* d = out.dx + (long)row * out.ld;
-  const int n_vec = in.n_cols / E, first = tile * RT * NV + t;
-  float k = 0.f, ks = 0.f, m = 0.f;
-  Word4 w[NV];
-  if (counted) {
-#pragma unroll
-    for (int u = 0; u < NV; ++u)
-      if (first + u * RT < n_vec) w[u] = Vec<T>::load(x + (long)(first + u * RT) * E);
-    const float2 st = in.stats[row];
-    k = label < in.n_cols ? coef[own] * up : NAN;
-    m = finite_or_zero(st.x);
-    ks = k / st.y;
-  }
-#pragma unroll
-  for (int u = 0; u < NV; ++u) {
-    const int i = first + u * RT;
-    if (i >= n_vec) break;
-    float v[E];
+  // Last rows first: they are what the pass that formed the statistics has left in the caches.  Where nothing is due
+  // mostly, the grid is smaller than the work and a block takes several pieces.
+  const long step = (long)gridDim.x * (JTVAE_BLOCK / RT);
+  long id = (long)in.n_rows * tiles - 1 - ((long)blockIdx.x * (JTVAE_BLOCK / RT) + threadIdx.x / RT);
+  for (; id >= 0; id -= step) {
+    const int row = (int)(id / tiles), tile = (int)(id - (long)row * tiles), t = threadIdx.x % RT;
+    const long label = in.labels[row];
+    const int own = in.owner ? in.owner[row] : row;
+    const bool counted = label >= 0 && own >= 0;
+    const T* x = in.x + (long)row * in.ld;
+    T* d = out.dx + (long)row * out.ld;
+    const Shape<T> shape(x, in.n_cols);
+    const int n_vec = shape.n_vec, first = tile * RT * NV + t;
+    float k = 0.f, ks = 0.f, m = 0.f;
+    Word4 w[NV];
     if (counted) {
-      Vec<T>::unpack(w[u], v);
-      softmax_grad<E>(v, (long)i * E, label, m, ks, k);
-    } else {
 #pragma unroll
-      for (int e = 0; e < E; ++e) v[e] = 0.f;
+      for (int u = 0; u < NV; ++u)
+        if (first + u * RT < n_vec)
+          w[u] = ONCE ? Vec<T>::load_once(x + shape.col(first + u * RT)) : Vec<T>::load(x + shape.col(first + u * RT));
+      const float2 st = in.stats[row];
+      k = label < in.n_cols ? coef[own] * up : NAN;
+      m = finite_or_zero(st.x);
+      ks = k / st.y;
     }
-    Vec<T>::store(d + (long)i * E, Vec<T>::pack(v));
-  }
-  if (tile == tiles - 1) {  // columns after the last whole vector, and the padding
-    for (long c = (long)n_vec * E + t; c < out.width; c += RT) {
-      float v = 0.f;
-      if (counted && c < in.n_cols) {
-        v = (float)x[c];
-        softmax_grad<1>(&v, c, label, m, ks, k);
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+      const int i = first + u * RT;
+      if (i >= n_vec) break;
+      float v[E];
+      if (counted) {
+        Vec<T>::unpack(w[u], v);
+        softmax_grad<E>(v, shape.col(i), label, m, ks, k);
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = 0.f;
       }
-      d[c] = (T)v;
+      Vec<T>::store(d + shape.col(i), Vec<T>::pack(v));
+    }
+    if (tile == 0) {  // single elements at the row's ends, and the padding
+      const int c = shape.extra(t);
+      if (c < in.n_cols) {
+        float v = 0.f;
+        if (counted) {
+          v = (float)x[c];
+          softmax_grad<1>(&v, c, label, m, ks, k);
+        }
+        d[c] = (T)v;
+      }
+      for (long p = in.n_cols + t; p < out.width; p += RT) d[p] = (T)0.f;
     }
   }
 }
@@ -585,14 +631,18 @@ int row_stats(const jtvae_logits_t* g, const int32_t* owner, float* stats, float
   return launch_status();
 }
 
-template <typename T, int RT, int NV>
+// The grid where the gradient mostly stands already: enough to fill the chip once.
+constexpr unsigned kIdleBlocks = 2048;
+
+template <typename T, int RT, int NV, bool ONCE>
 int launch_grad(const RowsIn<T>& in, const float* coef, const float* upstream, int unless_one, const GradOut<T>& out,
                 float* scaled, int n_scaled, hipStream_t s) {
   const int n_vec = in.n_cols / Vec<T>::E;
   const int tiles = n_vec > RT * NV ? (n_vec + RT * NV - 1) / (RT * NV) : 1;
-  const unsigned blocks = in.n_rows ? blocks_for((long)in.n_rows * tiles, JTVAE_BLOCK / RT) : 1;
-  hipLaunchKernelGGL((grad_kernel<T, RT, NV>), dim3(blocks), dim3(JTVAE_BLOCK), 0, s, in, coef, upstream, unless_one,
-                     tiles, out, scaled, n_scaled);
+  unsigned blocks = in.n_rows ? blocks_for((long)in.n_rows * tiles, JTVAE_BLOCK / RT) : 1;
+  if (unless_one && blocks > kIdleBlocks) blocks = kIdleBlocks;
+  hipLaunchKernelGGL((grad_kernel<T, RT, NV, ONCE>), dim3(blocks), dim3(JTVAE_BLOCK), 0, s, in, coef, upstream,
+                     unless_one, tiles, out, scaled, n_scaled);
   return launch_status();
 }
 
@@ -603,9 +653,13 @@ int row_grad(const jtvae_logits_t* g, const int32_t* owner, const float* stats, 
   const RowsIn<T> in = rows_in<T>(g, owner, (float*)stats, nullptr, nullptr);
   const GradOut<T> out = {(T*)dx, (long)ld_dx, (long)width};
   const int n_vec = g->n_cols / Vec<T>::E;
-  if (n_vec <= 128) return launch_grad<T, 64, 2>(in, coef, upstream, unless_one, out, scaled, n_scaled, s);
-  if (n_vec <= 256) return launch_grad<T, 64, 4>(in, coef, upstream, unless_one, out, scaled, n_scaled, s);
-  return launch_grad<T, 256, 4>(in, coef, upstream, unless_one, out, scaled, n_scaled, s);
+  if (n_vec <= 128) return launch_grad<T, 64, 2, false>(in, coef, upstream, unless_one, out, scaled, n_scaled, s);
+  if (n_vec <= 256) return launch_grad<T, 64, 4, false>(in, coef, upstream, unless_one, out, scaled, n_scaled, s);
+  // Logits beyond what the 256 MiB cache keeps pass through it without staying: 4096 x 128000 bf16 397 -> 373 us,
+  // 2048 x 50000 fp32 141 -> 135 us; small ones must not (64 x 30000 bf16 5.4 -> 6.7 us).
+  if ((double)g->n_rows * g->n_cols * sizeof(T) > 128e6)
+    return launch_grad<T, 256, 4, true>(in, coef, upstream, unless_one, out, scaled, n_scaled, s);
+  return launch_grad<T, 256, 4, false>(in, coef, upstream, unless_one, out, scaled, n_scaled, s);
 }
 
 // A policy row in one pass where its registers hold it; 1 when they do not.
