@@ -20,12 +20,15 @@ the GPU, the time loop disappears:
 * word and stop heads run as a few batch-wide dense products instead of being
   assembled step by step.
 
-Only ``forward`` (training) is provided: ``decode`` is a chemistry-driven host
-loop that needs RDKit and stays with the reference.
+``decode`` is a chemistry-driven host loop that needs RDKit and stays with the
+reference.  Beside ``forward`` (training) stand ``log_likelihood`` (the trees'
+log-probabilities, also as a frozen model's scoring pass) and ``preference_loss``
+(fine-tuning on pairs of trees), on the kernels of ``losses.py``.
 """
 from __future__ import annotations
 
 from dataclasses import dataclass
+from typing import NamedTuple
 
 import numpy as np
 import torch
@@ -35,6 +38,7 @@ import torch.nn.functional as F
 from . import graphprep
 from .jtnn_enc import _MessageGRUFunction
 from .linear import linear, table_linear
+from .losses import SequencePlan, preference_loss, sequence_log_probs
 from .nnutils import csr_gather_sum
 
 MAX_NB = 15  # fast_jtnn/jtnn_dec.py:9
@@ -164,6 +168,16 @@ def decoder_plan_from_arrays(wid, src, dst, roots) -> DecoderPlan:
                        pred_ctx=a["pred_ctx"].astype(np.int64), pred_target=a["pred_target"].astype(np.int64))
 
 
+class TraceScores(NamedTuple):
+    """What the decoder predicts along the traces of a batch, and what it should."""
+
+    plan: DecoderPlan
+    word_scores: torch.Tensor  # [n_pred, vocabulary] logits
+    word_targets: torch.Tensor  # [n_pred] word ids
+    stop_scores: torch.Tensor  # [n_stop] logit of going down
+    stop_targets: torch.Tensor  # [n_stop] 1 = go down, 0 = go back
+
+
 class JTNNDecoder(nn.Module):
     def __init__(self, vocab, hidden_size, latent_size, embedding):
         super(JTNNDecoder, self).__init__()
@@ -203,23 +217,25 @@ class JTNNDecoder(nn.Module):
                                          self.W_r.bias, self.U_r.weight, None, self.W_h.weight, self.W_h.bias,
                                          prep, torch.is_grad_enabled())
 
-    def forward(self, mol_batch, x_tree_vecs, jtenc_holder=None, sync=True):
-        """``jtenc_holder``: the junction-tree holder of the same batch, if the caller has it (JTNNVAE.forward
-        does): the trace tables then come from it natively and are kept with it; without it they are built
-        from the tree objects.  ``sync=False`` returns the two accuracies as 0-d device tensors instead of
-        Python floats (the caller fetches them together with its other scalars in one copy)."""
+    def _plan(self, mol_batch, jtenc_holder):
+        if jtenc_holder is None:
+            return decoder_plan(mol_batch)
+        key = jtenc_holder[3]
+        build = lambda: decoder_plan_from_holder(jtenc_holder)  # noqa: E731
+        plan = graphprep.cached_prep(key, ("decoder_plan",), build) if isinstance(key, torch.Tensor) else build()
+        if plan.n_trees != len(mol_batch):
+            raise ValueError("jtenc_holder describes %d trees, the batch has %d" % (plan.n_trees, len(mol_batch)))
+        return plan
+
+    def trace_scores(self, mol_batch, x_tree_vecs, jtenc_holder=None) -> TraceScores:
+        """Logits and targets of every word and stop prediction along the teacher-forced traces of the batch
+        (differentiable); row i of the words belongs to tree ``plan.pred_ctx[i]``, of the stops to ``plan.stop_ctx[i]``.
+        ``jtenc_holder``: as for ``forward``."""
         dev = self.W_z.weight.device
         if dev.type != "cuda":
             raise RuntimeError("fast_jtnn_hip.JTNNDecoder runs on an MI355X only (module is on %s); there is no "
                                "CPU path" % dev)
-        if jtenc_holder is None:
-            plan = decoder_plan(mol_batch)
-        else:
-            key = jtenc_holder[3]
-            build = lambda: decoder_plan_from_holder(jtenc_holder)  # noqa: E731
-            plan = graphprep.cached_prep(key, ("decoder_plan",), build) if isinstance(key, torch.Tensor) else build()
-            if plan.n_trees != len(mol_batch):
-                raise ValueError("jtenc_holder describes %d trees, the batch has %d" % (plan.n_trees, len(mol_batch)))
+        plan = self._plan(mol_batch, jtenc_holder)
         B, H = plan.n_trees, self.hidden_size
         with torch.cuda.device(dev):
             cache = plan.__dict__.setdefault("_device", {})
@@ -248,17 +264,58 @@ class JTNNDecoder(nn.Module):
             # word prediction: the root from a zero row, every child from the message that reaches it
             pred_hiddens = torch.cat([x_tree_vecs.new_zeros((B, H)), mess.index_select(0, pred_mess)], dim=0)
             pred_scores = self.aggregate(pred_hiddens, pred_ctx, x_tree_vecs, "word", pred_ctx32)
-            pred_loss = F.cross_entropy(pred_scores, pred_target, reduction="sum") / B
-            pred_acc = (pred_scores.argmax(dim=1) == pred_target).float().sum() / pred_target.nelement()
 
             # stop prediction: clique embedding and the sum of everything that has reached the node
             cur_o = csr_gather_sum(mess, stop_csr, stop_csr_t)
             # U_i(cat([embedding[stop_word], cur_o])): the embedding half as a per-word table       (jtnn_dec.py:160-163)
             stop_hiddens = table_linear(cur_o, self.embedding.weight, stop_word32, self.U_i, h_first=False, relu=True)
             stop_scores = self.aggregate(stop_hiddens, stop_ctx, x_tree_vecs, "stop", stop_ctx32).squeeze(-1)
+        return TraceScores(plan, pred_scores, pred_target, stop_scores, stop_target)
+
+    def forward(self, mol_batch, x_tree_vecs, jtenc_holder=None, sync=True):
+        """``jtenc_holder``: the junction-tree holder of the same batch, if the caller has it (JTNNVAE.forward
+        does): the trace tables then come from it natively and are kept with it; without it they are built
+        from the tree objects.  ``sync=False`` returns the two accuracies as 0-d device tensors instead of
+        Python floats (the caller fetches them together with its other scalars in one copy)."""
+        plan, pred_scores, pred_target, stop_scores, stop_target = self.trace_scores(mol_batch, x_tree_vecs, jtenc_holder)
+        B = plan.n_trees
+        with torch.cuda.device(pred_scores.device):
+            pred_loss = F.cross_entropy(pred_scores, pred_target, reduction="sum") / B
+            pred_acc = (pred_scores.argmax(dim=1) == pred_target).float().sum() / pred_target.nelement()
             stop_loss = F.binary_cross_entropy_with_logits(stop_scores, stop_target, reduction="sum") / B
             stop_acc = ((stop_scores >= 0).float() == stop_target).float().sum() / stop_target.nelement()
             if not sync:
                 return pred_loss, stop_loss, pred_acc, stop_acc
             accs = torch.stack([pred_acc, stop_acc]).tolist()  # one host sync for both
         return pred_loss, stop_loss, accs[0], accs[1]
+
+    def _sequences(self, plan, device, what):
+        """Which tree every prediction belongs to, kept with the decoder plan."""
+        cache = plan.__dict__.setdefault("_sequences", {})
+        key = (str(device), what)
+        if key not in cache:
+            cache[key] = SequencePlan(plan.pred_ctx if what == "word" else plan.stop_ctx, plan.n_trees, device)
+        return cache[key]
+
+    def _stop_log_probs(self, s: TraceScores):
+        """[n_trees] log-probability of the stop decisions: a decision is a choice between the logits 0 and score."""
+        two = torch.stack([torch.zeros_like(s.stop_scores), s.stop_scores], dim=1)
+        return sequence_log_probs(two, s.stop_targets.long(), self._sequences(s.plan, two.device, "stop"))
+
+    def log_likelihood(self, mol_batch, x_tree_vecs, jtenc_holder=None):
+        """[n_trees] log-probability of every tree of the batch given its latent vector: the sum over its word and stop
+        predictions (``forward`` returns minus the mean of the same sums).  Differentiable; under ``torch.no_grad()`` the
+        scoring pass of a frozen model, e.g. the reference of ``preference_loss``."""
+        s = self.trace_scores(mol_batch, x_tree_vecs, jtenc_holder)
+        words = sequence_log_probs(s.word_scores, s.word_targets, self._sequences(s.plan, s.word_scores.device, "word"))
+        return words + self._stop_log_probs(s)
+
+    def preference_loss(self, mol_batch, x_tree_vecs, pairs, ref_log_probs, beta=0.1, label_smoothing=0.0,
+                        jtenc_holder=None):
+        """Loss of learning which of two trees is preferred: ``pairs`` are host integers [P, 2], (preferred, other)
+        position in the batch, ``ref_log_probs`` [n_trees] what ``log_likelihood`` of the frozen reference model gave.
+        Returns ``losses.PreferenceLoss``; its ``log_probs`` are the present log-likelihoods."""
+        s = self.trace_scores(mol_batch, x_tree_vecs, jtenc_holder)
+        words = SequencePlan(s.plan.pred_ctx, s.plan.n_trees, s.word_scores.device, pairs=pairs)
+        return preference_loss(s.word_scores, s.word_targets, words, ref_log_probs, beta=beta,
+                               label_smoothing=label_smoothing, other_log_probs=self._stop_log_probs(s))

@@ -68,16 +68,32 @@ class StepResult:
     error: Optional[str] = None
 
 
+OPTIMIZERS = ("adam", "adamw", "adamw8")
+
+
 class Trainer:
     """One model replica on one GPU (or the CPU oracle in tests): ``step(batch)`` is one iteration of the
     reference's inner loop."""
 
     def __init__(self, model: nn.Module, sched: Schedule = None, save_dir: str = None, conditional: bool = False,
-                 total_step: int = 0, log=print):
+                 total_step: int = 0, log=print, optimizer: str = "adam", weight_decay: float = 0.0):
+        """``optimizer``: "adam" (the reference's), or "adamw" / "adamw8", the package's AdamW with 32- or 8-bit states,
+        which clips inside its step: ``.grad`` then keeps the unclipped gradient."""
+        if optimizer not in OPTIMIZERS:
+            raise ValueError("optimizer %r is none of %s" % (optimizer, ", ".join(OPTIMIZERS)))
+        if optimizer == "adam" and weight_decay:
+            raise ValueError("weight_decay goes with optimizer adamw or adamw8")
         self.model, self.sched, self.save_dir, self.conditional = model, sched or Schedule(), save_dir, conditional
         self.params = [p for p in model.parameters() if p.requires_grad]
         self.bucket = parallel.FlatGradBucket(self.params)  # one buffer for the gradient all-reduce
-        self.optimizer = torch.optim.Adam(self.params, lr=self.sched.lr)  # vae_train.py:73-74
+        self.clips = optimizer != "adam"  # the optimizer's own step does
+        if self.clips:
+            from .optim import AdamW
+
+            self.optimizer = AdamW(self.params, lr=self.sched.lr, weight_decay=weight_decay,
+                                   state_bits=8 if optimizer == "adamw8" else 32, max_norm=self.sched.clip_norm)
+        else:
+            self.optimizer = torch.optim.Adam(self.params, lr=self.sched.lr)  # vae_train.py:73-74
         self.scheduler = torch.optim.lr_scheduler.ExponentialLR(self.optimizer, self.sched.anneal_rate)
         self.beta = self.sched.beta
         self.total_step = total_step
@@ -118,11 +134,20 @@ class Trainer:
             self.log("Batch %d failed%s" % (self.total_step, "" if err is None else "\n" + err))
             return StepResult(False, error=err)
         self.bucket.all_reduce_mean(force=self.force_collective)
-        nn.utils.clip_grad_norm_(self.params, self.sched.clip_norm)
+        if self.clips:
+            self.optimizer.max_norm = self.sched.clip_norm
+        else:
+            nn.utils.clip_grad_norm_(self.params, self.sched.clip_norm)
         self.optimizer.step()
         res = StepResult(True, float(loss.detach()), metrics)
         self._after_step(res)
         return res
+
+    def _clipped_norm(self) -> float:
+        """Norm of the gradient the step was taken with."""
+        if self.clips:
+            return min(float(self.optimizer.grad_norm), self.sched.clip_norm)
+        return grad_norm(self.model)
 
     def _after_step(self, res: StepResult) -> None:
         s, m = self.sched, res.metrics
@@ -132,13 +157,13 @@ class Trainer:
             if self.conditional:  # vae_train_prop.py:129-139
                 items = ["Loss: %.2f" % res.loss, " Beta: %.5f" % self.beta] + \
                         [" %s: %.3f" % (k, v) for k, v in m.items()] + \
-                        ["PNorm: %.3f" % param_norm(self.model), "GNorm: %.3f" % grad_norm(self.model)]
+                        ["PNorm: %.3f" % param_norm(self.model), "GNorm: %.3f" % self._clipped_norm()]
                 self.log(",".join(items))
             else:  # vae_train.py:112-132
                 mt = self.meters / s.print_iter
                 self.log("[%d] Loss: %.3f,Beta: %.3f,KL: %.2f, Word: %.2f, Topo: %.2f, Assm: %.2f, PNorm: %.2f, "
                          "GNorm: %.2f" % (self.total_step, res.loss, self.beta, mt[0], mt[1], mt[2], mt[3],
-                                          param_norm(self.model), grad_norm(self.model)))
+                                          param_norm(self.model), self._clipped_norm()))
         if self.total_step % s.print_iter == 0:
             self.meters *= 0
         if self.total_step % s.save_iter == 0:

@@ -175,3 +175,26 @@ def test_c_entry_points_refuse_before_launch():
     assert lib.jtvae_adamw_step(None, 0, 0.0, None, None, None) == 0
     assert step(-1, 0.0) == K.E_SHAPE and step(1, -1.0) == K.E_RANGE and step(1, float("nan")) == K.E_RANGE
     assert step(1, 1.0, partials=None) == K.E_NULL and step(1, 1.0, out=None) == K.E_NULL
+
+
+def test_trainer_optimizers_refused():
+    from fast_jtnn_hip import trainer
+
+    m = torch.nn.Linear(3, 2)
+    with pytest.raises(ValueError, match="is none of"):
+        trainer.Trainer(m, optimizer="sgd")
+    with pytest.raises(ValueError, match="weight_decay"):
+        trainer.Trainer(m, weight_decay=0.1)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        trainer.Trainer(m, optimizer="adamw")
+    assert isinstance(trainer.Trainer(m).optimizer, torch.optim.Adam)
+
+
+def test_decoder_entry_points_refuse_cpu():
+    from fast_jtnn_hip import JTNNDecoder, synthetic
+
+    d = JTNNDecoder(synthetic.FakeVocab(5), 16, 4, torch.nn.Embedding(5, 16))
+    for call in (lambda: d.log_likelihood([], torch.zeros(0, 4)), lambda: d.trace_scores([], torch.zeros(0, 4)),
+                 lambda: d.preference_loss([], torch.zeros(0, 4), [[0, 1]], torch.zeros(2))):
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            call()

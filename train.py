@@ -11,7 +11,8 @@ the holders of its own share with the native tensorizers.  ``--train synthetic:N
 molecules from the in-package generator; ``--train flat:<file.npz>`` reads a data set in flat form
 (``fast_jtnn_hip.flat.save_shard``: atoms, bonds, feature bytes, tree neighbour lists, candidates - turning SMILES
 into those arrays needs RDKit and stays with the caller).  ``--vocab`` is a vocabulary file (one entry per line; only its
-length is used for synthetic data) or an integer.
+length is used for synthetic data) or an integer.  ``--optimizer adamw`` / ``adamw8`` step with the package's AdamW
+(decoupled ``--weight_decay``, clip inside the step, states in 32 or 8 bits) in place of the reference's Adam.
 """
 import argparse
 import os
@@ -40,6 +41,8 @@ def parse_args(argv=None):
     ap.add_argument("--depthG", type=int, default=3)
     ap.add_argument("--lr", type=float, default=1e-3)
     ap.add_argument("--clip_norm", type=float, default=50.0)
+    ap.add_argument("--optimizer", choices=["adam", "adamw", "adamw8"], default="adam")
+    ap.add_argument("--weight_decay", type=float, default=0.0, help="decoupled decay (adamw, adamw8)")
     ap.add_argument("--beta", type=float, default=0.0)
     ap.add_argument("--step_beta", type=float, default=0.002)
     ap.add_argument("--max_beta", type=float, default=1.0)
@@ -137,7 +140,7 @@ def main(argv=None):
                              anneal_iter=args.anneal_iter, kl_anneal_iter=args.kl_anneal_iter,
                              print_iter=args.print_iter, save_iter=args.save_iter)
     tr = trainer.Trainer(model, sched, save_dir=args.save_dir, conditional=args.conditional,
-                         total_step=args.load_epoch)
+                         total_step=args.load_epoch, optimizer=args.optimizer, weight_decay=args.weight_decay)
     torch.manual_seed(1234 + rank)  # every rank draws its own rsample noise
     import torch as _t
 
