@@ -120,8 +120,8 @@ struct Shape {
     n_cols = cols;
   }
   __device__ __forceinline__ int col(int i) const { return head + i * Vec<T>::E; }
-  __device__ __forceinline__ int extra(int t) const {  // >= n_cols: none
-    return t < head ? t : n_vec * Vec<T>::E + t;
+  __device__ __forceinline__ unsigned extra(int t) const {  // >= n_cols: none (a row may have 2^31 - 1 columns)
+    return t < head ? (unsigned)t : (unsigned)(n_vec * Vec<T>::E) + (unsigned)t;
   }
 };
 
@@ -175,7 +175,7 @@ template <typename T>
 struct RowsIn {
   const T* x;
   long ld;
-  int n_rows, n_cols;
+  int first, n_rows, n_cols;  // a launch takes the rows [first, n_rows)
   Labels labels;
   const int* owner;
   float2* stats;
@@ -204,7 +204,7 @@ template <typename T, int BLOCK>
 __global__ __launch_bounds__(BLOCK) void stats_kernel(RowsIn<T> in) {
   constexpr int E = Vec<T>::E, U = 4;
   __shared__ RowStat part[BLOCK / 64];
-  const int row = blockIdx.x;
+  const int row = in.first + blockIdx.x;
   const long label = in.labels[row];
   if (!counts(in, row, label)) {
     if (threadIdx.x == 0) finish_row(in, row, label, false, RowStat{0.f, 1.f});
@@ -229,8 +229,8 @@ __global__ __launch_bounds__(BLOCK) void stats_kernel(RowsIn<T> in) {
     Vec<T>::unpack(Vec<T>::load(r + shape.col(i)), v);
     take<E>(st, v);
   }
-  const int c = shape.extra(threadIdx.x);
-  if (c < in.n_cols) {
+  const unsigned c = shape.extra(threadIdx.x);
+  if (c < (unsigned)in.n_cols) {
     const float v = (float)r[c];
     take<1>(st, &v);
   }
@@ -269,26 +269,32 @@ enum { kStats = 0, kPolicy = 1 };
 // arithmetic of a row's end is done by one lane per row, side by side.
 template <typename T, int RT, int R, int NV, int MODE>
 __global__ __launch_bounds__(RT* R, NV > 8 ? 4 : RT == 64 && NV == 8 ? 6 : 8) void rows_kernel(RowsIn<T> in, PolicyIn policy, float* __restrict__ coef,
-                                                     double* __restrict__ terms, GradOut<T> out) {
+                                                     double* __restrict__ terms, long n_terms, GradOut<T> out) {
   constexpr int E = Vec<T>::E, W = RT / 64;
+  // long policy rows are read once and for all: past the caches (8192 x 32000 bf16 201 -> 191 us); short ones lose by it
+  // (20480 x 780 fp32 36 -> 40 us)
+  constexpr bool kOnce = MODE == kPolicy && RT > 64;
   __shared__ RowStat part[R * W];
   __shared__ float4 end[R];  // m, s, coefficient, counted
   const int r = threadIdx.x / RT, t = threadIdx.x % RT;
-  const int row = blockIdx.x * R + r;
-  const bool there = row < in.n_rows;
+  const long first = in.first + (long)blockIdx.x * R;
+  const int row = (int)(first + r);
+  const bool there = first + r < in.n_rows;
   const long label = there ? in.labels[row] : -1;
   const bool counted = there && counts(in, row, label);
   const T* x = in.x + (long)row * in.ld;
   const Shape<T> shape(x, in.n_cols);
-  const int n_vec = shape.n_vec, c_one = shape.extra(t);
+  const int n_vec = shape.n_vec;
+  const unsigned c_one = shape.extra(t);
   Word4 w[NV];
   float one = -INFINITY;
   RowStat st = {-INFINITY, 0.f};
   if (counted) {
 #pragma unroll
     for (int u = 0; u < NV; ++u)
-      if (t + u * RT < n_vec) w[u] = Vec<T>::load(x + shape.col(t + u * RT));
-    if (c_one < in.n_cols) one = (float)x[c_one];
+      if (t + u * RT < n_vec)
+        w[u] = kOnce ? Vec<T>::load_once(x + shape.col(t + u * RT)) : Vec<T>::load(x + shape.col(t + u * RT));
+    if (c_one < (unsigned)in.n_cols) one = (float)x[c_one];
     // the maximum of all that a lane holds first, so that every value takes one exponential
     st.m = one;
 #pragma unroll
@@ -315,8 +321,8 @@ __global__ __launch_bounds__(RT* R, NV > 8 ? 4 : RT == 64 && NV == 8 ? 6 : 8) vo
   }
   __syncthreads();
   if (threadIdx.x < R) {
-    const int i = threadIdx.x, mine = blockIdx.x * R + i;
-    if (mine < in.n_rows) {
+    const int i = threadIdx.x, mine = (int)(first + i);
+    if (first + i < in.n_rows) {
       const long l = in.labels[mine];
       const bool c = counts(in, mine, l);
       RowStat s = {0.f, 1.f};
@@ -330,8 +336,8 @@ __global__ __launch_bounds__(RT* R, NV > 8 ? 4 : RT == 64 && NV == 8 ? 6 : 8) vo
         if (c) p = policy_row(policy, mine, lp);
         coef[mine] = p.coef;
         terms[mine] = p.loss;
-        terms[(long)in.n_rows + mine] = p.kl;
-        terms[2L * in.n_rows + mine] = p.clipped;
+        terms[n_terms + mine] = p.kl;
+        terms[2 * n_terms + mine] = p.clipped;
         end[i] = make_float4(s.m, s.s, l < in.n_cols ? p.coef : NAN, 0.f);
       }
     }
@@ -357,7 +363,7 @@ __global__ __launch_bounds__(RT* R, NV > 8 ? 4 : RT == 64 && NV == 8 ? 6 : 8) vo
       }
       Vec<T>::store(d + shape.col(i), Vec<T>::pack(v));
     }
-    if (c_one < in.n_cols) {
+    if (c_one < (unsigned)in.n_cols) {
       float v = 0.f;
       if (counted) {
         v = one;
@@ -385,9 +391,10 @@ __global__ __launch_bounds__(JTVAE_BLOCK) void grad_kernel(RowsIn<T> in, const f
   // Last rows first: they are what the pass that formed the statistics has left in the caches.  Where nothing is due
   // mostly, the grid is smaller than the work and a block takes several pieces.
   const long step = (long)gridDim.x * (JTVAE_BLOCK / RT);
-  long id = (long)in.n_rows * tiles - 1 - ((long)blockIdx.x * (JTVAE_BLOCK / RT) + threadIdx.x / RT);
+  long id = (long)(in.n_rows - in.first) * tiles - 1 - ((long)blockIdx.x * (JTVAE_BLOCK / RT) + threadIdx.x / RT);
   for (; id >= 0; id -= step) {
-    const int row = (int)(id / tiles), tile = (int)(id - (long)row * tiles), t = threadIdx.x % RT;
+    const long r = id / tiles;
+    const int row = in.first + (int)r, tile = (int)(id - r * tiles), t = threadIdx.x % RT;
     const long label = in.labels[row];
     const int own = in.owner ? in.owner[row] : row;
     const bool counted = label >= 0 && own >= 0;
@@ -422,8 +429,8 @@ __global__ __launch_bounds__(JTVAE_BLOCK) void grad_kernel(RowsIn<T> in, const f
       Vec<T>::store(d + shape.col(i), Vec<T>::pack(v));
     }
     if (tile == 0) {  // single elements at the row's ends, and the padding
-      const int c = shape.extra(t);
-      if (c < in.n_cols) {
+      const unsigned c = shape.extra(t);
+      if (c < (unsigned)in.n_cols) {
         float v = 0.f;
         if (counted) {
           v = (float)x[c];
@@ -458,12 +465,13 @@ __global__ __launch_bounds__(JTVAE_BLOCK) void sequence_sums_kernel(Sequences q,
                                                                     const float* __restrict__ other,
                                                                     double* __restrict__ sums64,
                                                                     float* __restrict__ sums) {
-  const int seq = (int)(((long)blockIdx.x * JTVAE_BLOCK + threadIdx.x) >> 6), lane = threadIdx.x & 63;
-  if (seq >= q.n_seq) return;
-  const double acc = sequence_sum(q, lp64, other, seq, lane);
-  if (lane == 0) {
-    if (sums64) sums64[seq] = acc;
-    sums[seq] = (float)acc;
+  const int lane = threadIdx.x & 63;
+  for (long seq = ((long)blockIdx.x * JTVAE_BLOCK + threadIdx.x) >> 6; seq < q.n_seq; seq += (long)gridDim.x * (JTVAE_BLOCK / 64)) {
+    const double acc = sequence_sum(q, lp64, other, (int)seq, lane);
+    if (lane == 0) {
+      if (sums64) sums64[seq] = acc;
+      sums[seq] = (float)acc;
+    }
   }
 }
 
@@ -497,7 +505,7 @@ __global__ __launch_bounds__(kPairBlock) void preference_kernel(Sequences q, Pre
     __syncthreads();
   }
   double acc = 0.0;
-  for (int p = threadIdx.x; p < q.n_pairs; p += kPairBlock) {
+  for (long p = threadIdx.x; p < q.n_pairs; p += kPairBlock) {
     const int2 ab = q.pairs[p];
     const double d =
         in.beta * ((sums64[ab.x] - (double)in.ref[ab.x]) - (sums64[ab.y] - (double)in.ref[ab.y]));
@@ -517,7 +525,7 @@ __global__ __launch_bounds__(kPairBlock) void preference_kernel(Sequences q, Pre
     for (int w = 0; w < kPairBlock / 64; ++w) t += part[w];
     *loss = (float)(in.scale * t);
   }
-  for (int s = threadIdx.x; s < q.n_seq; s += kPairBlock) {
+  for (long s = threadIdx.x; s < q.n_seq; s += kPairBlock) {
     double c = 0.0;
     for (int i = q.pair_ptr[s]; i < q.pair_ptr[s + 1]; ++i) {
       const int e = q.pair_list[i];
@@ -532,8 +540,9 @@ __global__ __launch_bounds__(JTVAE_BLOCK) void policy_rows_kernel(PolicyIn in, c
                                                                   Labels labels, int n_rows,
                                                                   float* __restrict__ coef,
                                                                   double* __restrict__ terms) {
-  const int row = blockIdx.x * JTVAE_BLOCK + threadIdx.x;
-  if (row >= n_rows) return;
+  const long at = (long)blockIdx.x * JTVAE_BLOCK + threadIdx.x;
+  if (at >= n_rows) return;
+  const int row = (int)at;
   PolicyRow o = {0.0, 0.0, 0.0, 0.f};
   if (labels[row] >= 0) o = policy_row(in, row, lp64[row]);
   coef[row] = o.coef;
@@ -550,7 +559,7 @@ __global__ __launch_bounds__(kPairBlock) void sum_terms_kernel(const double* __r
   double a = 0.0, b = 0.0, c = 0.0;
   const double *kls = terms + n_rows, *cut = kls + n_rows;
 #pragma unroll 8
-  for (int i = threadIdx.x; i < n_rows; i += kPairBlock) {
+  for (long i = threadIdx.x; i < n_rows; i += kPairBlock) {
     a += terms[i];
     b += kls[i];
     c += cut[i];
@@ -585,6 +594,12 @@ int check_logits(const jtvae_logits_t* g) {
   return 0;
 }
 
+// A wave per sequence; beyond a million of them a wave takes several.
+unsigned sum_blocks(int n_seq) {
+  const unsigned b = grid_for((long)n_seq * 64);
+  return b < (1u << 18) ? b : 1u << 18;
+}
+
 int check_sequences(const jtvae_sequences_t* q, int n_rows, bool pairs) {
   if (!q) return JTVAE_E_NULL;
   if (q->n_seq < 0 || (pairs && q->n_pairs < 0)) return JTVAE_E_SHAPE;
@@ -599,18 +614,41 @@ Sequences sequences_of(const jtvae_sequences_t* q) {
 
 template <typename T>
 RowsIn<T> rows_in(const jtvae_logits_t* g, const int32_t* owner, float* stats, float* lp32, double* lp64) {
-  return RowsIn<T>{(const T*)g->x, (long)g->ld, g->n_rows, g->n_cols, Labels{g->labels, g->label_bits}, owner,
+  return RowsIn<T>{(const T*)g->x, (long)g->ld, 0, g->n_rows, g->n_cols, Labels{g->labels, g->label_bits}, owner,
                    (float2*)stats, lp32, lp64};
 }
 
 inline unsigned blocks_for(long items, int per) { return (unsigned)((items + per - 1) / per); }
 
+// Calls launch(part of the rows, how many) so that no grid has more than 2^31 work-items (the limit is 2^32).
+template <typename T, typename F>
+int for_row_parts(RowsIn<T> in, long lanes_per_row, F launch) {
+  const int n = in.n_rows;
+  const long most = lanes_per_row < (1L << 31) ? (1L << 31) / lanes_per_row : 1;
+  for (long r0 = 0; r0 < n; r0 += most) {
+    in.first = (int)r0;
+    in.n_rows = (int)(n - r0 < most ? n : r0 + most);
+    launch(in, in.n_rows - in.first);
+    int rc = launch_status();
+    if (rc) return rc;
+  }
+  return 0;
+}
+
 template <typename T, int RT, int R, int NV, int MODE>
-int launch_rows(const RowsIn<T>& in, const PolicyIn& p, float* coef, double* terms, const GradOut<T>& out,
+int launch_rows(const RowsIn<T>& rows, const PolicyIn& p, float* coef, double* terms, const GradOut<T>& out,
                 hipStream_t s) {
-  hipLaunchKernelGGL((rows_kernel<T, RT, R, NV, MODE>), dim3(blocks_for(in.n_rows, R)), dim3(RT * R), 0, s, in, p, coef,
-                     terms, out);
-  return launch_status();
+  return for_row_parts(rows, RT, [&](const RowsIn<T>& in, int n) {
+    hipLaunchKernelGGL((rows_kernel<T, RT, R, NV, MODE>), dim3(blocks_for(n, R)), dim3(RT * R), 0, s, in, p, coef, terms,
+                       (long)rows.n_rows, out);
+  });
+}
+
+template <typename T, int BLOCK>
+int launch_stats(const RowsIn<T>& rows, hipStream_t s) {
+  return for_row_parts(rows, BLOCK, [&](const RowsIn<T>& in, int n) {
+    hipLaunchKernelGGL((stats_kernel<T, BLOCK>), dim3(n), dim3(BLOCK), 0, s, in);
+  });
 }
 
 // Statistics.  Rows of up to 512 vectors (8 KiB) sit in a wave's registers, eight waves side by side; longer ones are
@@ -624,25 +662,26 @@ int row_stats(const jtvae_logits_t* g, const int32_t* owner, float* stats, float
   const GradOut<T> no_grad = {};
   if (n_vec <= 128) return launch_rows<T, 64, 8, 2, kStats>(in, none, nullptr, nullptr, no_grad, s);
   if (n_vec <= 512) return launch_rows<T, 64, 8, 8, kStats>(in, none, nullptr, nullptr, no_grad, s);
-  if (g->n_rows >= 1024)
-    hipLaunchKernelGGL((stats_kernel<T, 256>), dim3(g->n_rows), dim3(256), 0, s, in);
-  else
-    hipLaunchKernelGGL((stats_kernel<T, 1024>), dim3(g->n_rows), dim3(1024), 0, s, in);
-  return launch_status();
+  return g->n_rows >= 1024 ? launch_stats<T, 256>(in, s) : launch_stats<T, 1024>(in, s);
 }
 
 // The grid where the gradient mostly stands already: enough to fill the chip once.
 constexpr unsigned kIdleBlocks = 2048;
 
 template <typename T, int RT, int NV, bool ONCE>
-int launch_grad(const RowsIn<T>& in, const float* coef, const float* upstream, int unless_one, const GradOut<T>& out,
+int launch_grad(const RowsIn<T>& rows, const float* coef, const float* upstream, int unless_one, const GradOut<T>& out,
                 float* scaled, int n_scaled, hipStream_t s) {
-  const int n_vec = in.n_cols / Vec<T>::E;
+  const int n_vec = rows.n_cols / Vec<T>::E;
   const int tiles = n_vec > RT * NV ? (n_vec + RT * NV - 1) / (RT * NV) : 1;
-  unsigned blocks = in.n_rows ? blocks_for((long)in.n_rows * tiles, JTVAE_BLOCK / RT) : 1;
-  if (unless_one && blocks > kIdleBlocks) blocks = kIdleBlocks;
-  hipLaunchKernelGGL((grad_kernel<T, RT, NV, ONCE>), dim3(blocks), dim3(JTVAE_BLOCK), 0, s, in, coef, upstream,
-                     unless_one, tiles, out, scaled, n_scaled);
+  const auto launch = [&](const RowsIn<T>& in, int n) {
+    unsigned blocks = n ? blocks_for((long)n * tiles, JTVAE_BLOCK / RT) : 1;
+    if (unless_one && blocks > kIdleBlocks) blocks = kIdleBlocks;
+    hipLaunchKernelGGL((grad_kernel<T, RT, NV, ONCE>), dim3(blocks), dim3(JTVAE_BLOCK), 0, s, in, coef, upstream,
+                       unless_one, tiles, out, scaled, n_scaled);
+    n_scaled = 0;  // once is enough
+  };
+  if (rows.n_rows) return for_row_parts(rows, (long)RT * tiles, launch);
+  launch(rows, 0);
   return launch_status();
 }
 
@@ -658,8 +697,8 @@ int row_grad(const jtvae_logits_t* g, const int32_t* owner, const float* stats, 
   // Logits beyond what the 256 MiB cache keeps pass through it without staying: 4096 x 128000 bf16 397 -> 373 us,
   // 2048 x 50000 fp32 141 -> 135 us; small ones must not (64 x 30000 bf16 5.4 -> 6.7 us).
   if ((double)g->n_rows * g->n_cols * sizeof(T) > 128e6)
-    return launch_grad<T, 256, 4, true>(in, coef, upstream, unless_one, out, scaled, n_scaled, s);
-  return launch_grad<T, 256, 4, false>(in, coef, upstream, unless_one, out, scaled, n_scaled, s);
+    return launch_grad<T, 256, 2, true>(in, coef, upstream, unless_one, out, scaled, n_scaled, s);
+  return launch_grad<T, 256, 2, false>(in, coef, upstream, unless_one, out, scaled, n_scaled, s);
 }
 
 // A policy row in one pass where its registers hold it; 1 when they do not.
@@ -744,7 +783,7 @@ int jtvae_sequence_log_probs(const jtvae_logits_t* logits, const jtvae_sequences
   if (workspace_bytes < jtvae_sequence_log_probs_workspace_bytes(logits->n_rows)) return JTVAE_E_WORKSPACE;
   double* lp64 = (double*)workspace;
   JT_CHECK(jtvae_label_log_probs(logits, sequences->row_seq, stats, nullptr, lp64, stream));
-  hipLaunchKernelGGL(sequence_sums_kernel, dim3(grid_for((long)sequences->n_seq * 64)), dim3(JTVAE_BLOCK), 0,
+  hipLaunchKernelGGL(sequence_sums_kernel, dim3(sum_blocks(sequences->n_seq)), dim3(JTVAE_BLOCK), 0,
                      (hipStream_t)stream, sequences_of(sequences), lp64, nullptr, nullptr, sums);
   return launch_status();
 }
@@ -779,7 +818,7 @@ int jtvae_preference_loss(const jtvae_logits_t* logits, const jtvae_sequences_t*
                        margins, dmargin, coef);
     return launch_status();
   }
-  hipLaunchKernelGGL(sequence_sums_kernel, dim3(grid_for((long)n_seq * 64)), dim3(JTVAE_BLOCK), 0, s, q, lp64,
+  hipLaunchKernelGGL(sequence_sums_kernel, dim3(sum_blocks(n_seq)), dim3(JTVAE_BLOCK), 0, s, q, lp64,
                      in.other, sums64, sums);
   JT_CHECK(launch_status());
   hipLaunchKernelGGL(preference_kernel<false>, dim3(1), dim3(kPairBlock), 0, s, q, in, lp64, sums64, sums, loss,

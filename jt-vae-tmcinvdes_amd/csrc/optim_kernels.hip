@@ -25,19 +25,41 @@ inline int launch_status() {
   return e == hipSuccess ? 0 : (int)e;
 }
 
-// N consecutive elements from i, at the type's own alignment (the hardware takes a 16-byte access at any address); WHOLE:
-// all of them exist, else those from n on read as zero and are not written.
+// N consecutive elements from i, at the type's own alignment (the hardware takes an access of 16 bytes at any address).
+// WHOLE: all of them exist, else those from n on read as zero and are not written.  ONCE: past the caches - a step
+// touches every byte once, and no chip-wide cache holds a model's states until the next one.
+template <int BYTES>
+struct Words;
+template <>
+struct Words<16> {
+  typedef unsigned at4 __attribute__((ext_vector_type(4), aligned(4)));
+  typedef unsigned at2 __attribute__((ext_vector_type(4), aligned(2)));
+};
+template <>
+struct Words<8> {
+  typedef unsigned at4 __attribute__((ext_vector_type(2), aligned(4)));
+  typedef unsigned at2 __attribute__((ext_vector_type(2), aligned(2)));
+};
+template <typename T, int N, bool TWO = sizeof(T) == 2>
+struct Run {
+  using type = typename Words<N * sizeof(T)>::at4;
+};
 template <typename T, int N>
-struct __attribute__((packed, aligned(sizeof(T)))) Run {
-  T at[N];
+struct Run<T, N, true> {
+  using type = typename Words<N * sizeof(T)>::at2;
 };
 
-template <bool WHOLE, int N, typename T>
+template <bool WHOLE, bool ONCE, int N, typename T>
 __device__ __forceinline__ void load(const T* p, long i, long n, float v[N]) {
   if constexpr (WHOLE) {
-    const Run<T, N> r = *(const Run<T, N>*)(p + i);
+    using R = typename Run<T, N>::type;
+    R r;
+    if constexpr (ONCE) r = __builtin_nontemporal_load((const R*)(p + i));
+    else r = *(const R*)(p + i);
+    T h[N];
+    __builtin_memcpy(h, &r, sizeof(h));
 #pragma unroll
-    for (int k = 0; k < N; ++k) v[k] = (float)r.at[k];
+    for (int k = 0; k < N; ++k) v[k] = (float)h[k];
   } else {
 #pragma unroll
     for (int k = 0; k < N; ++k) v[k] = i + k < n ? (float)p[i + k] : 0.f;
@@ -46,10 +68,13 @@ __device__ __forceinline__ void load(const T* p, long i, long n, float v[N]) {
 template <bool WHOLE, int N, typename T>
 __device__ __forceinline__ void store(T* p, long i, long n, const float v[N]) {
   if constexpr (WHOLE) {
-    Run<T, N> r;
+    using R = typename Run<T, N>::type;
+    T h[N];
 #pragma unroll
-    for (int k = 0; k < N; ++k) r.at[k] = (T)v[k];
-    *(Run<T, N>*)(p + i) = r;
+    for (int k = 0; k < N; ++k) h[k] = (T)v[k];
+    R r;
+    __builtin_memcpy(&r, h, sizeof(h));
+    __builtin_nontemporal_store(r, (R*)(p + i));
   } else {
 #pragma unroll
     for (int k = 0; k < N; ++k)
@@ -64,7 +89,7 @@ __device__ __forceinline__ double chunk_squares(const T* g, long base, long n) {
 #pragma unroll
   for (int u = 0; u < JTVAE_ADAMW_CHUNK / (kBlock * N); ++u) {
     float v[N], s = 0.f;
-    load<WHOLE, N>(g, base + (u * kBlock + threadIdx.x) * N, n, v);
+    load<WHOLE, false, N>(g, base + (u * kBlock + threadIdx.x) * N, n, v);
 #pragma unroll
     for (int k = 0; k < N; ++k) s = fmaf(v[k], v[k], s);
     acc += (double)s;
@@ -143,56 +168,44 @@ struct Hyper {
   const float *lr_device, *grad_scale;
 };
 
-// e4m3 values of a lane, four to a 32-bit word, and back with the format's rounding to nearest even.
-template <int N>
-__device__ __forceinline__ void unpack_e4m3(const uint8_t q[N], float v[N]) {
-#pragma unroll
-  for (int k = 0; k < N; k += 4) {
-    int w;
-    __builtin_memcpy(&w, q + k, 4);
-    auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
-    v[k] = lo[0];
-    v[k + 1] = lo[1];
-    v[k + 2] = hi[0];
-    v[k + 3] = hi[1];
-  }
+// The four e4m3 values of a word, and back with the format's rounding to nearest even.
+__device__ __forceinline__ void unpack_e4m3(unsigned w, float v[4]) {
+  auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+  v[0] = lo[0];
+  v[1] = lo[1];
+  v[2] = hi[0];
+  v[3] = hi[1];
 }
-template <int N>
-__device__ __forceinline__ void pack_e4m3(const float v[N], uint8_t q[N]) {
-#pragma unroll
-  for (int k = 0; k < N; k += 4) {
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[k], v[k + 1], 0, false);
-    w = __builtin_amdgcn_cvt_pk_fp8_f32(v[k + 2], v[k + 3], w, true);
-    __builtin_memcpy(q + k, &w, 4);
-  }
+__device__ __forceinline__ unsigned pack_e4m3(const float v[4]) {
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], w, true);
+  return (unsigned)w;
 }
 
-// Largest finite magnitude among the values of the lanes that share a scale: a scale is not lost to one element that
-// overflowed.
-template <int N>
-__device__ __forceinline__ float block_top(const float v[N]) {
+// Largest finite magnitude of a wave's 256 values: a scale is not lost to one element that overflowed.
+__device__ __forceinline__ float block_top(const float v[4]) {
   float t = 0.f;
 #pragma unroll
-  for (int k = 0; k < N; ++k) {
+  for (int k = 0; k < 4; ++k) {
     const float a = fabsf(v[k]);
     t = fmaxf(t, a < INFINITY ? a : 0.f);
   }
 #pragma unroll
-  for (int off = kGroup / N / 2; off > 0; off >>= 1) t = fmaxf(t, __shfl_xor(t, off, 64));
+  for (int off = 32; off > 0; off >>= 1) t = fmaxf(t, __shfl_xor(t, off, 64));
   return t;
 }
 
-template <bool ROOT, int N>
-__device__ __forceinline__ void quantise(const float v[N], float top, uint8_t q[N]) {
+template <bool ROOT>
+__device__ __forceinline__ unsigned quantise(const float v[4], float top) {
   const float inv = top > kSmallest ? kTop / top : 0.f;
-  float x[N];
+  float x[4];
 #pragma unroll
-  for (int k = 0; k < N; ++k) {
+  for (int k = 0; k < 4; ++k) {
     float y = fminf(fmaxf(v[k] * inv, -kTop), kTop);
     if (ROOT) y = y > 0.f ? fmaxf(y, 0x1p-9f) : y;
     x[k] = fabsf(v[k]) < INFINITY ? y : NAN;
   }
-  pack_e4m3<N>(x, q);
+  return pack_e4m3(x);
 }
 
 // sqrt on the hardware unit (1 ulp), with what it would flush brought into its range first.
@@ -206,113 +219,87 @@ struct Step {
   float keep, rate, eps, beta1, one_m_beta1, beta2, one_m_beta2, grad_scale, bias2;
 };
 
-// N elements of a tensor from `at`: loads, the update, and what goes back.  8-bit states: kGroup / N neighbouring lanes
-// share a scale.
-template <typename T, bool MASTER, int BITS, bool WHOLE, int N>
-struct Piece {
-  float g[N], w[N], m[N], v[N];
-  uint8_t qm[N], qr[N];
-  float sm, sr;
-
-  __device__ __forceinline__ void fetch(const jtvae_adamw_tensor_t& t, const T* grad, long at) {
-    load<WHOLE, N>(grad, at, t.n, g);
-    if constexpr (MASTER) load<WHOLE, N>((const float*)t.master, at, t.n, w);
-    else load<WHOLE, N>((const T*)t.param, at, t.n, w);
-    if constexpr (BITS == 32) {
-      load<WHOLE, N>((const float*)t.exp_avg, at, t.n, m);
-      load<WHOLE, N>((const float*)t.second, at, t.n, v);
-    } else {
-      // the states' buffers are padded to whole blocks
-      __builtin_memcpy(qm, __builtin_assume_aligned((const uint8_t*)t.exp_avg + at, N), N);
-      __builtin_memcpy(qr, __builtin_assume_aligned((const uint8_t*)t.second + at, N), N);
-      sm = t.exp_avg_scale[at / kGroup];
-      sr = t.second_scale[at / kGroup];
-    }
-  }
-
-  __device__ __forceinline__ void update(const jtvae_adamw_tensor_t& t, const Step& s, long at) {
-    float r[N];
-    if constexpr (BITS == 8) {
-      unpack_e4m3<N>(qm, m);
-      unpack_e4m3<N>(qr, r);
-#pragma unroll
-      for (int k = 0; k < N; ++k) {
-        m[k] *= sm;
-        r[k] *= sr;
-        v[k] = r[k] * r[k];
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const float x = g[k] * s.grad_scale;
-      m[k] = s.beta1 * m[k] + s.one_m_beta1 * x;
-      v[k] = s.beta2 * v[k] + s.one_m_beta2 * (x * x);
-      r[k] = root(v[k]);
-      // reciprocal on the hardware unit (1 ulp): the update is off by 2^-22 of itself, below half an ulp of w
-      w[k] = w[k] * s.keep - s.rate * (m[k] * __builtin_amdgcn_rcpf(r[k] * s.bias2 + s.eps));
-      // a 16-bit parameter is the 32-bit value rounded: the compiler must not round the sum to 16 bits by itself
-      if constexpr (sizeof(T) == 2) asm("" : "+v"(w[k]));
-    }
-    if constexpr (MASTER) store<WHOLE, N>(t.master, at, t.n, w);
-    store<WHOLE, N>((T*)t.param, at, t.n, w);
-    if constexpr (BITS == 32) {
-      store<WHOLE, N>((float*)t.exp_avg, at, t.n, m);
-      store<WHOLE, N>((float*)t.second, at, t.n, v);
-    } else {
-      if constexpr (!WHOLE) {  // the padding after the last element stays zero
-#pragma unroll
-        for (int k = 0; k < N; ++k)
-          if (at + k >= t.n) m[k] = r[k] = 0.f;
-      }
-      const float tm = block_top<N>(m), tr = block_top<N>(r);
-      quantise<false, N>(m, tm, qm);
-      quantise<true, N>(r, tr, qr);
-      __builtin_memcpy(__builtin_assume_aligned((uint8_t*)t.exp_avg + at, N), qm, N);
-      __builtin_memcpy(__builtin_assume_aligned((uint8_t*)t.second + at, N), qr, N);
-      if ((threadIdx.x & (kGroup / N - 1)) == 0) {
-        t.exp_avg_scale[at / kGroup] = tm > kSmallest ? tm / kTop : 0.f;
-        t.second_scale[at / kGroup] = tr > kSmallest ? tr / kTop : 0.f;
-      }
-    }
-  }
-};
-
+// The four elements of a tensor from `at`.  8-bit states: a wave's 256 elements are a block, which shares a scale; its
+// buffers are padded to whole blocks.
 template <typename T, bool MASTER, int BITS, bool WHOLE>
-__device__ __forceinline__ void update_chunk(const jtvae_adamw_tensor_t& t, const T* g, long base, const Step& s) {
-  constexpr int N = BITS == 8 ? 8 : 4, U = 2, kStride = kBlock * N;
-  static_assert(JTVAE_ADAMW_CHUNK % (kStride * U) == 0, "whole rounds");
+__device__ __forceinline__ void update(const jtvae_adamw_tensor_t& t, const T* grad, const Step& s, long at) {
+  float g[4], w[4], m[4], v[4], r[4];
+  load<WHOLE, true, 4>(grad, at, t.n, g);
+  if constexpr (MASTER) load<WHOLE, true, 4>((const float*)t.master, at, t.n, w);
+  else load<WHOLE, true, 4>((const T*)t.param, at, t.n, w);
+  if constexpr (BITS == 32) {
+    load<WHOLE, true, 4>((const float*)t.exp_avg, at, t.n, m);
+    load<WHOLE, true, 4>((const float*)t.second, at, t.n, v);
+  } else {
+    const unsigned qm = __builtin_nontemporal_load((const unsigned*)((const uint8_t*)t.exp_avg + at));
+    const unsigned qr = __builtin_nontemporal_load((const unsigned*)((const uint8_t*)t.second + at));
+    const float sm = t.exp_avg_scale[at / kGroup], sr = t.second_scale[at / kGroup];
+    unpack_e4m3(qm, m);
+    unpack_e4m3(qr, r);
 #pragma unroll
-  for (int i = 0; i < JTVAE_ADAMW_CHUNK; i += kStride * U) {
-    Piece<T, MASTER, BITS, WHOLE, N> p[U];
-    bool there[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const long at = base + i + u * kStride + threadIdx.x * N;
-      // the same for all lanes that share a scale: the first element of their block
-      there[u] = WHOLE || at / kGroup * kGroup < t.n;
-      if (there[u]) p[u].fetch(t, g, at);
+    for (int k = 0; k < 4; ++k) {
+      m[k] *= sm;
+      r[k] *= sr;
+      v[k] = r[k] * r[k];
     }
+  }
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (there[u]) p[u].update(t, s, base + i + u * kStride + threadIdx.x * N);
+  for (int k = 0; k < 4; ++k) {
+    const float x = g[k] * s.grad_scale;
+    m[k] = s.beta1 * m[k] + s.one_m_beta1 * x;
+    v[k] = s.beta2 * v[k] + s.one_m_beta2 * (x * x);
+    r[k] = root(v[k]);
+    // reciprocal on the hardware unit (1 ulp): the update is off by 2^-22 of itself, below half an ulp of w
+    w[k] = w[k] * s.keep - s.rate * (m[k] * __builtin_amdgcn_rcpf(r[k] * s.bias2 + s.eps));
+    // a 16-bit parameter is the 32-bit value rounded: the compiler must not round the sum to 16 bits by itself
+    if constexpr (sizeof(T) == 2) asm("" : "+v"(w[k]));
+  }
+  if constexpr (MASTER) store<WHOLE, 4>(t.master, at, t.n, w);
+  store<WHOLE, 4>((T*)t.param, at, t.n, w);
+  if constexpr (BITS == 32) {
+    store<WHOLE, 4>((float*)t.exp_avg, at, t.n, m);
+    store<WHOLE, 4>((float*)t.second, at, t.n, v);
+  } else {
+    if constexpr (!WHOLE) {  // the padding after the last element stays zero
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (at + k >= t.n) m[k] = r[k] = 0.f;
+    }
+    const float tm = block_top(m), tr = block_top(r);
+    __builtin_nontemporal_store(quantise<false>(m, tm), (unsigned*)((uint8_t*)t.exp_avg + at));
+    __builtin_nontemporal_store(quantise<true>(r, tr), (unsigned*)((uint8_t*)t.second + at));
+    if ((threadIdx.x & 63) == 0) {
+      t.exp_avg_scale[at / kGroup] = tm > kSmallest ? tm / kTop : 0.f;
+      t.second_scale[at / kGroup] = tr > kSmallest ? tr / kTop : 0.f;
+    }
   }
 }
+
+// One round of a block's lanes, four elements each.  Bound by memory: 28 bytes per fp32 element with 32-bit states, 16
+// per bf16 element with a copy and 8-bit states.  A copy on this card reaches 6.2-6.6 TB/s with one 16-byte access per
+// lane and block and 4.2 with eight - the fewer bytes a block holds, the closer together the places the chip works on
+// at a time - and so it is here: rounds of 1024 elements past the caches take 1396 us for 477 M bf16 elements with
+// 8-bit states, chunks of 4096 through the caches 1642 (the norm's pass included).
+constexpr int kRound = kBlock * 4, kRounds = JTVAE_ADAMW_CHUNK / kRound;
+static_assert(JTVAE_ADAMW_CHUNK % kRound == 0 && kRound % kGroup == 0, "whole rounds of whole blocks");
 
 template <typename T, bool MASTER, int BITS>
 __global__ __launch_bounds__(kBlock) void adamw_kernel(const jtvae_adamw_tensor_t* __restrict__ tensors,
                                                        const int2* __restrict__ chunks, long first_chunk, Grads grads,
                                                        const float2* __restrict__ bias, Hyper h) {
-  const int2 c = chunks[first_chunk + blockIdx.x];
+  const int2 c = chunks[first_chunk + blockIdx.x / kRounds];
   const T* g = (const T*)grads.at[c.x - grads.first];
   if (!g) return;
   const jtvae_adamw_tensor_t t = tensors[c.x];
+  const long base = (long)c.y * JTVAE_ADAMW_CHUNK + (blockIdx.x % kRounds) * kRound;
+  const long at = base + threadIdx.x * 4;
+  if (at / kGroup * kGroup >= t.n) return;  // the same for the lanes of a wave: the first element of their block
   const float2 b = bias[c.x];
   const float lr = h.lr_device ? *h.lr_device : h.lr;
   const Step s = {1.f - lr * h.decay, lr * b.x,      h.eps, h.beta1, h.one_m_beta1, h.beta2, h.one_m_beta2,
                   h.grad_scale ? *h.grad_scale : 1.f, b.y};
-  const long base = (long)c.y * JTVAE_ADAMW_CHUNK;
-  if (base + JTVAE_ADAMW_CHUNK <= t.n) update_chunk<T, MASTER, BITS, true>(t, g, base, s);
-  else update_chunk<T, MASTER, BITS, false>(t, g, base, s);
+  if (base + kRound <= t.n) update<T, MASTER, BITS, true>(t, g, s, at);
+  else update<T, MASTER, BITS, false>(t, g, s, at);
 }
 
 int check_group(const jtvae_adamw_group_t* g) {
@@ -326,19 +313,22 @@ int check_group(const jtvae_adamw_group_t* g) {
   return 0;
 }
 
-// Calls launch(grads, first chunk, number of chunks) for runs of at most JTVAE_ADAMW_MAX_TENSORS tensors.
+// Calls launch(grads, first chunk, number of chunks) for runs of at most JTVAE_ADAMW_MAX_TENSORS tensors and of as many
+// chunks as a grid may have work-items for (2^32).
 template <typename F>
 int for_runs(const jtvae_adamw_group_t* g, F launch) {
+  constexpr int64_t kMost = (int64_t)1 << 21;
   for (int t0 = 0; t0 < g->n_tensors; t0 += JTVAE_ADAMW_MAX_TENSORS) {
     const int cnt = g->n_tensors - t0 < JTVAE_ADAMW_MAX_TENSORS ? g->n_tensors - t0 : JTVAE_ADAMW_MAX_TENSORS;
-    const int64_t c0 = g->chunk_ptr[t0], nc = g->chunk_ptr[t0 + cnt] - c0;
-    if (nc <= 0) continue;
     Grads a;
     a.first = t0;
     for (int i = 0; i < cnt; ++i) a.at[i] = g->grads[t0 + i];
-    launch(a, (long)c0, (unsigned)nc);
-    int rc = launch_status();
-    if (rc) return rc;
+    const int64_t end = g->chunk_ptr[t0 + cnt];
+    for (int64_t c0 = g->chunk_ptr[t0]; c0 < end; c0 += kMost) {
+      launch(a, (long)c0, (unsigned)(end - c0 < kMost ? end - c0 : kMost));
+      int rc = launch_status();
+      if (rc) return rc;
+    }
   }
   return 0;
 }
@@ -347,10 +337,10 @@ template <typename T, bool MASTER>
 int step(const jtvae_adamw_group_t* g, const Hyper& h, hipStream_t s) {
   return for_runs(g, [&](const Grads& a, long c0, unsigned nc) {
     if (g->state_bits == 32)
-      hipLaunchKernelGGL((adamw_kernel<T, MASTER, 32>), dim3(nc), dim3(kBlock), 0, s, g->tensors,
+      hipLaunchKernelGGL((adamw_kernel<T, MASTER, 32>), dim3(nc * kRounds), dim3(kBlock), 0, s, g->tensors,
                          (const int2*)g->chunks, c0, a, (const float2*)g->bias, h);
     else
-      hipLaunchKernelGGL((adamw_kernel<T, MASTER, 8>), dim3(nc), dim3(kBlock), 0, s, g->tensors,
+      hipLaunchKernelGGL((adamw_kernel<T, MASTER, 8>), dim3(nc * kRounds), dim3(kBlock), 0, s, g->tensors,
                          (const int2*)g->chunks, c0, a, (const float2*)g->bias, h);
   });
 }

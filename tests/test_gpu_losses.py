@@ -551,3 +551,30 @@ def test_captured_and_replayed(n, v, dtype):
         torch.cuda.synchronize()
         for i, (a, b) in enumerate(zip(outs, want)):
             assert torch.equal(a, b), (k, i)
+
+
+def test_more_rows_than_one_launch_takes():
+    """68 million rows of two columns: more work-items than a grid may have, so several launches."""
+    from fast_jtnn_hip import policy_loss, token_log_probs
+
+    n = 68_000_000
+    x = torch.zeros(n, 2, dtype=torch.float16, device="cuda")
+    labels = torch.zeros(n, dtype=torch.int32, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(1)
+    spots = [slice(0, 1000), slice(n // 2 - 500, n // 2 + 500), slice((1 << 25) - 500, (1 << 25) + 500), slice(n - 1000, n)]
+    for s in spots:
+        x[s] = torch.randn(1000, 2, generator=g, device="cuda").half()
+        labels[s] = torch.randint(0, 2, (1000,), generator=g, device="cuda").int()
+    x.requires_grad_()
+    coef = torch.ones(n, device="cuda")
+    lp = token_log_probs(x, labels)
+    (d,) = torch.autograd.grad(lp, x, coef)
+    out = policy_loss(x, labels, torch.full((n,), -0.5, device="cuda"), coef, clip=(0.9, 9.0))
+    (e,) = torch.autograd.grad(out.loss, x)
+    for s in spots:
+        want, soft, dist = exact(x[s], labels[s])
+        check_lp(lp[s], want, 2)
+        check_lp(out.log_probs[s], want, 2)
+        check_grad(d[s], soft, dist, labels[s].long(), coef[s], torch.float16)
+        check_grad(e[s], soft, dist, labels[s].long(), -torch.exp(want + 0.5).float(), torch.float16)
+    assert abs(float(out.loss) + math.exp(0.5) * float(torch.exp(lp.double()).sum())) <= 1e-5 * n
