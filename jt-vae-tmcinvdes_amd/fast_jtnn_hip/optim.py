@@ -102,18 +102,14 @@ class _Group:
 
     def gather_grads(self):
         """Fills the address list; (parameters with a gradient, tensors to keep alive until the launches)."""
-        keep, at = [], []
-        for p in self.params:
-            g = p.grad
-            if g is None:
-                at.append(None)
-                continue
-            if not g.is_contiguous():
-                g = g.contiguous()
-                keep.append(g)
-            at.append(g.data_ptr())
-        self.grads[:] = at
-        return (self.params if None not in at else [p for p, a in zip(self.params, at) if a is not None]), keep
+        grads, have, keep = [p.grad for p in self.params], self.params, []
+        missing = [g is None for g in grads]
+        if any(missing):
+            have = [p for p, m in zip(self.params, missing) if not m]
+        if not all([g is None or g.is_contiguous() for g in grads]):
+            grads = keep = [None if g is None else g.contiguous() for g in grads]
+        self.grads[:] = [None if g is None else g.data_ptr() for g in grads]
+        return have, keep
 
     def args(self, hyper):
         lr = hyper["lr"]
@@ -149,8 +145,8 @@ class AdamW(torch.optim.Optimizer):
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, master=True,
                  max_norm=None):
         self._bound = []
-        self.max_norm = self._check_norm(max_norm)
         self._norm = None
+        self.max_norm = self._check_norm(max_norm)
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       master=master))
 
