@@ -11,7 +11,9 @@ preferred, learning from rewards of sampled ones - needs the log-probability of 
 
 Logits are [N, V] in fp32, fp16 or bf16, rows at any stride; labels are [N] int32 or int64, a negative label leaves its
 row out (log-probability 0, gradient 0, its logits are never read).  A label >= V gives NaN.  Gradients come back in the
-logits' type and layout.  Statistics are fp32, sums over a sequence fp64; no atomics, so results repeat bit for bit.
+logits' type and layout, and are differentiable once.  Statistics are fp32, sums over a sequence fp64; no atomics, so
+results repeat bit for bit.  Every call only enqueues work on the current stream and may be captured; a captured plan
+lives as long as the graph.
 """
 from __future__ import annotations
 
@@ -349,7 +351,8 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, plan: SequencePl
         D_p = beta ((S - ref_log_probs)[preferred] - (S - ref_log_probs)[other]),
 
     the loss is ``scale * sum_p -(1 - label_smoothing) log sigmoid(D_p) - label_smoothing log sigmoid(-D_p)``; ``scale``
-    defaults to one over the number of pairs.  Differentiable in ``logits`` and ``other_log_probs``."""
+    defaults to one over the number of pairs.  Differentiable in ``logits`` and ``other_log_probs``; ``ref_log_probs``
+    [plan.n_seq] are constants, read in fp32."""
     what = "preference_loss"
     _check(what, logits, labels)
     _check_plan(what, plan, logits, pairs=True)
@@ -366,7 +369,7 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, plan: SequencePl
 
 class _PolicyLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, labels, old, adv, ref, weights, lo, hi, kl_coef, scale):
+    def forward(ctx, logits, labels, old, adv, ref, weights, lo, hi, kl_coef, scale, want_grad):
         x, dev, n = _rows(logits), logits.device, logits.shape[0]
         with _guard(dev):
             old, adv, ref, weights = (_fp32(t) for t in (old, adv, ref, weights))
@@ -375,7 +378,7 @@ class _PolicyLoss(torch.autograd.Function):
             nbytes = K.policy_loss_workspace_bytes(n)
             ctx.ws, (stats, coef, ws) = _scratch(dev, n, (n + 1) // 2, nbytes // 8)
             # a row's coefficient depends on that row alone: its gradient is made while the row is in registers
-            d, ld = _grad_rows(x) if ctx.needs_input_grad[0] else (None, 0)
+            d, ld = _grad_rows(x) if want_grad else (None, 0)
             ctx.arg = g, _ = _arg(x, labels)
             policy = K.Policy(old.data_ptr(), adv.data_ptr(), K.ptr(ref), K.ptr(weights), lo, hi, kl_coef, scale)
             K.policy_loss(g, policy, stats, lp.data_ptr(), coef, loss.data_ptr(), kl.data_ptr(), clipped.data_ptr(),
@@ -390,7 +393,7 @@ class _PolicyLoss(torch.autograd.Function):
     @_differentiable_once
     def backward(ctx, dloss, *_):
         if dloss is None:
-            return (None,) * 10
+            return (None,) * 11
         x, labels = ctx.saved_tensors
         d, ctx.gradient = ctx.gradient, None
         fresh = d is not None  # else a second pass through the graph: the first one's gradient has been given away
@@ -404,7 +407,7 @@ class _PolicyLoss(torch.autograd.Function):
             # a fresh gradient stands as it is where the upstream factor is 1, which only the device knows
             K.label_log_probs_bwd(_again(ctx, x, labels), None, stats, stats + 8 * x.shape[0], up.data_ptr(), d.data_ptr(), ld, ld,
                                   unless_one=int(fresh))
-        return (d,) + (None,) * 9
+        return (d,) + (None,) * 10
 
 
 def policy_loss(logits: torch.Tensor, labels: torch.Tensor, old_log_probs: torch.Tensor, advantages: torch.Tensor,
@@ -416,7 +419,9 @@ def policy_loss(logits: torch.Tensor, labels: torch.Tensor, old_log_probs: torch
         loss = scale * sum over rows of weights (kl_coef k - min(r A, min(max(r, 1 - clip), 1 + clip) A)).
 
     ``clip`` is one number or (low, high); without ``ref_log_probs`` there is no KL term (``kl_coef`` must be 0).  Rows
-    with a negative label do not count; ``weights`` (default 1) carry masks and means.  Differentiable in ``logits``."""
+    with a negative label do not count; ``weights`` (default 1) carry masks and means.  Differentiable in ``logits``; the
+    other inputs are constants.  The gradient is made along with the loss, for a factor of one on it: a factor is best
+    given as ``scale`` (another one in the backward pass is right too, and makes the gradient a second time)."""
     what = "policy_loss"
     _check(what, logits, labels)
     given = dict(old_log_probs=old_log_probs, advantages=advantages, ref_log_probs=ref_log_probs, weights=weights)
@@ -431,4 +436,4 @@ def policy_loss(logits: torch.Tensor, labels: torch.Tensor, old_log_probs: torch
         raise ValueError("%s: kl_coef needs ref_log_probs" % what)
     _on_device(what, logits, labels=labels, **given)
     return PolicyLoss(*_PolicyLoss.apply(logits, labels, old_log_probs, advantages, ref_log_probs, weights, lo, hi,
-                                         kl_coef, scale))
+                                         kl_coef, scale, logits.requires_grad and torch.is_grad_enabled()))

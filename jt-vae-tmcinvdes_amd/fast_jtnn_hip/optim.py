@@ -85,10 +85,10 @@ class _Group:
         addresses = [p.data_ptr() for p in self.params]
         if addresses == self.addresses:
             return
-        for p in self.params:
-            if p.device != self.device or p.dtype != self.dtype or not p.is_contiguous():
-                raise RuntimeError("AdamW: a parameter changed its device, type or layout after the optimizer was "
-                                   "built; build it again")
+        for p, n in zip(self.params, self.numels):
+            if p.device != self.device or p.dtype != self.dtype or p.numel() != n or not p.is_contiguous():
+                raise RuntimeError("AdamW: a parameter changed its device, type, size or layout after the optimizer "
+                                   "was built; build it again")
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW: the parameters' addresses must be known before a capture; make one step first")
         items = (K.AdamwTensor * len(self.params))()
@@ -106,8 +106,10 @@ class _Group:
         missing = [g is None for g in grads]
         if any(missing):
             have = [p for p, m in zip(self.params, missing) if not m]
-        if not all([g is None or g.is_contiguous() for g in grads]):
-            grads = keep = [None if g is None else g.contiguous() for g in grads]
+        if [n if g is None else g.numel() for g, n in zip(grads, self.numels)] != self.numels:
+            raise RuntimeError("AdamW: a gradient has another size than its parameter had when the optimizer was built")
+        if not all([g is None or (g.dtype is self.dtype and g.is_contiguous()) for g in grads]):
+            grads = keep = [None if g is None else g.to(self.dtype).contiguous() for g in grads]
         self.grads[:] = [None if g is None else g.data_ptr() for g in grads]
         return have, keep
 

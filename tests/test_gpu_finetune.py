@@ -48,6 +48,25 @@ def test_log_likelihood_is_minus_the_training_losses():
         assert abs(float(ll[i]) + float(w + st)) <= RTOL * abs(float(w + st)), i
 
 
+def test_log_likelihood_of_single_node_trees():
+    from fast_jtnn_hip import synthetic
+
+    g, _ = _seeded_training_problem(1, 2, 8.0, V=9)
+    g.H, g.L = 32, 8
+    hip = make_hip_model(g, "cuda")
+    mol = synthetic.make_mol(np.random.RandomState(0), 6.0, 1.0, 4, 8)
+    trees = [synthetic.Tree([synthetic.TreeNode(1, w)], mol) for w in (2, 5)]
+    synthetic.set_batch_nodeID(trees)
+    zt = torch.from_numpy(np.random.RandomState(1).standard_normal((2, 4)).astype(np.float32)).cuda().requires_grad_()
+    ll = hip.decoder.log_likelihood(trees, zt)
+    word, stop, _, _ = hip.decoder(trees, zt)
+    assert ll.shape == (2,) and abs(float(ll.sum()) + 2 * float(word + stop)) <= 1e-5 * 2 * float(word + stop)
+    r = hip.decoder.preference_loss(trees, zt, [[0, 1]], ll.detach())
+    assert abs(float(r.loss) - math.log(2.0)) <= 1e-6
+    r.loss.backward()
+    assert torch.isfinite(zt.grad).all()
+
+
 def test_preference_loss_of_the_decoder():
     """Against the same loss written with torch's operations on the log-likelihoods: value, margins, every gradient."""
     B = 10

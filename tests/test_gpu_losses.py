@@ -578,3 +578,103 @@ def test_more_rows_than_one_launch_takes():
         check_grad(d[s], soft, dist, labels[s].long(), coef[s], torch.float16)
         check_grad(e[s], soft, dist, labels[s].long(), -torch.exp(want + 0.5).float(), torch.float16)
     assert abs(float(out.loss) + math.exp(0.5) * float(torch.exp(lp.double()).sum())) <= 1e-5 * n
+
+
+def test_nothing_is_made_for_a_gradient_nobody_wants():
+    from fast_jtnn_hip import policy_loss
+
+    x, labels = make(2000, 30000, torch.bfloat16, 3)
+    f = torch.full((2000,), -2.0, device="cuda")
+    x.requires_grad_()
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    with torch.no_grad():
+        a = policy_loss(x, labels, f, f)
+    assert not a.loss.requires_grad and torch.cuda.max_memory_allocated() - before < 4 << 20
+    b = policy_loss(x, labels, f, f)
+    assert torch.equal(a.loss, b.loss) and torch.equal(a.log_probs, b.log_probs)
+
+
+def test_inputs_on_the_host_are_refused():
+    from fast_jtnn_hip import SequencePlan, policy_loss, preference_loss, token_log_probs
+
+    x, labels = make(4, 9, torch.float32, 2)
+    plan = SequencePlan([0, 0, 1, 1], 2, "cuda", pairs=[[0, 1]])
+    f, two = torch.zeros(4, device="cuda"), torch.zeros(2, device="cuda")
+    for call in (lambda: token_log_probs(x, labels.cpu()), lambda: preference_loss(x, labels, plan, two.cpu()),
+                 lambda: preference_loss(x, labels, plan, two, other_log_probs=two.cpu()),
+                 lambda: policy_loss(x, labels, f, f.cpu()), lambda: policy_loss(x, labels, f, f, weights=f.cpu())):
+        with pytest.raises(RuntimeError, match="logits are on"):
+            call()
+
+
+def test_calls_are_timed_like_the_others():
+    from fast_jtnn_hip import AdamW, SequencePlan, preference_loss
+    from fast_jtnn_hip import _capi as K
+
+    x, labels = make(40, 500, torch.float16, 2)
+    x = torch.nn.Parameter(x.clone())
+    plan = SequencePlan(np.arange(40) % 2, 2, "cuda", pairs=[[0, 1]])
+    opt = AdamW([x], max_norm=1.0)
+    with K.KernelTimer() as t:
+        preference_loss(x, labels, plan, torch.zeros(2, device="cuda")).loss.backward()
+        opt.step()
+    got = t.summary()
+    assert set(got) == {"preference_loss", "label_log_probs_bwd", "adamw_step"}
+    assert got["label_log_probs_bwd"]["bytes"] >= 2 * 40 * 500 * 2
+    assert got["adamw_step"]["bytes"] >= 40 * 500 * (2 * 2 + 8 + 16)
+
+
+def test_saved_tensors_that_come_back_elsewhere():
+    """Hooks that move saved tensors to the host and back: the backward pass reads them where they are now."""
+    from fast_jtnn_hip import SequencePlan, policy_loss, preference_loss, token_log_probs
+
+    x, labels = make(30, 700, torch.float32, 5)
+    plan = SequencePlan(np.arange(30) % 2, 2, "cuda", pairs=[[0, 1]])
+    two, f = torch.zeros(2, device="cuda"), torch.full((30,), -1.0, device="cuda")
+    for call in (lambda y: token_log_probs(y, labels).sum(), lambda y: preference_loss(y, labels, plan, two).loss,
+                 lambda y: policy_loss(y, labels, f, f).loss * 2):
+        got = []
+        for moved in (False, True):
+            leaf = x.clone().requires_grad_()
+            if moved:
+                with torch.autograd.graph.save_on_cpu():
+                    loss = call(leaf * 1.0)
+            else:
+                loss = call(leaf * 1.0)
+            junk = torch.full((40, 900), 7.0, device="cuda")  # takes the place of what was freed
+            loss.backward()
+            got.append(leaf.grad)
+            del junk
+        assert torch.equal(*got)
+
+
+def test_two_threads_at_once():
+    """Calls from two host threads on streams of their own."""
+    import threading
+
+    from fast_jtnn_hip import policy_loss
+
+    x, labels = make(300, 5000, torch.bfloat16, 6)
+    f = torch.full((300,), -2.0, device="cuda")
+    leaf = x.clone().requires_grad_()
+    want = torch.autograd.grad(policy_loss(leaf, labels, f, f).loss, leaf)[0]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(seed):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            y = x.clone().requires_grad_()
+            for _ in range(20):
+                r = policy_loss(y, labels, f, f)
+                (d,) = torch.autograd.grad(r.loss, y)
+                s.synchronize()
+                if not torch.equal(d, want):
+                    bad.append(seed)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not bad

@@ -346,7 +346,38 @@ def test_moved_parameters_and_master_refresh():
     opt.step()
     assert torch.allclose(p.float(), torch.full_like(p.float(), 2.75), atol=1e-2)
     p.data = p.data.float()
-    with pytest.raises(RuntimeError, match="changed its device, type or layout"):
+    with pytest.raises(RuntimeError, match="changed its device, type, size or layout"):
+        opt.step()
+
+
+def test_gradients_of_another_type_or_size():
+    """A gradient type of its own is converted; a parameter whose data was exchanged for another size is refused."""
+    from fast_jtnn_hip import AdamW
+
+    p = torch.nn.Parameter(torch.ones(700, device="cuda", dtype=torch.bfloat16))
+    if hasattr(p, "grad_dtype"):
+        p.grad_dtype = None
+        p.grad = torch.ones(700, device="cuda")
+        opt = AdamW([p], lr=0.25, weight_decay=0.0)
+        opt.step()
+        assert (p.detach() == 0.75).all()
+    for new in (torch.ones(9, device="cuda"), torch.ones(5000, device="cuda")):
+        q = torch.nn.Parameter(torch.ones(300, device="cuda"))
+        q.grad = torch.ones(300, device="cuda")
+        opt = AdamW([q])
+        opt.step()
+        q.data = new
+        with pytest.raises(RuntimeError, match="size"):  # the old gradient's size, the new parameter's address
+            opt.step()
+        q.grad = torch.ones_like(q)
+        with pytest.raises(RuntimeError, match="size"):
+            opt.step()
+    q = torch.nn.Parameter(torch.ones(300, device="cuda"))
+    opt = AdamW([q])
+    opt.step()
+    q.data = q.data[:100]  # the same address
+    q.grad = torch.ones_like(q)
+    with pytest.raises(RuntimeError, match="size"):
         opt.step()
 
 
