@@ -176,7 +176,8 @@ def _number(what, name, v, lo, hi=float("inf")):
 _NOTHING = contextlib.nullcontext()
 
 
-def _guard(device):
+def guard(device):
+    """The device as the current one; nothing is switched where it is already."""
     return _NOTHING if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
@@ -234,7 +235,7 @@ class _TokenLogProbs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, labels):
         x, dev, n = _rows(logits), logits.device, logits.shape[0]
-        with _guard(dev):
+        with guard(dev):
             lp = torch.empty((n,), dtype=torch.float32, device=dev)
             ctx.ws, (stats,) = _scratch(dev, n)
             ctx.arg = g, _ = _arg(x, labels)
@@ -246,7 +247,7 @@ class _TokenLogProbs(torch.autograd.Function):
     @_differentiable_once
     def backward(ctx, dlp):
         x, labels = ctx.saved_tensors
-        with _guard(x.device):
+        with guard(x.device):
             coef = dlp.float().contiguous()
             d, ld = _grad_rows(x)
             K.label_log_probs_bwd(_again(ctx, x, labels), None, ctx.ws.data_ptr(), coef.data_ptr(), None, d.data_ptr(), ld, ld)
@@ -264,7 +265,7 @@ class _SequenceLogProbs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, labels, plan):
         x, dev, n = _rows(logits), logits.device, logits.shape[0]
-        with _guard(dev):
+        with guard(dev):
             plan.on_current_stream()
             sums = torch.empty((plan.n_seq,), dtype=torch.float32, device=dev)
             ctx.ws, (stats, ws) = _scratch(dev, n, n)
@@ -278,7 +279,7 @@ class _SequenceLogProbs(torch.autograd.Function):
     @_differentiable_once
     def backward(ctx, dsums):
         x, labels = ctx.saved_tensors
-        with _guard(x.device):
+        with guard(x.device):
             coef = dsums.float().contiguous()
             d, ld = _grad_rows(x)
             g, keep = _arg(x, labels)
@@ -301,7 +302,7 @@ class _PreferenceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, other, labels, plan, ref, beta, smoothing, scale):
         x, dev, n, S, P = _rows(logits), logits.device, logits.shape[0], plan.n_seq, plan.n_pairs
-        with _guard(dev):
+        with guard(dev):
             plan.on_current_stream()
             oth, ref = _fp32(other), _fp32(ref)
             sums = torch.empty((S,), dtype=torch.float32, device=dev)
@@ -326,7 +327,7 @@ class _PreferenceLoss(torch.autograd.Function):
         plan, d, dother = ctx.plan, None, None
         stats = ctx.ws.data_ptr()
         coef = stats + 8 * x.shape[0]
-        with _guard(x.device):
+        with guard(x.device):
             up = dloss.float()
             if ctx.needs_input_grad[1]:
                 dother = torch.empty((plan.n_seq,), dtype=torch.float32, device=x.device)
@@ -371,7 +372,7 @@ class _PolicyLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, labels, old, adv, ref, weights, lo, hi, kl_coef, scale, want_grad):
         x, dev, n = _rows(logits), logits.device, logits.shape[0]
-        with _guard(dev):
+        with guard(dev):
             old, adv, ref, weights = (_fp32(t) for t in (old, adv, ref, weights))
             lp = torch.empty((n,), dtype=torch.float32, device=dev)
             loss, kl, clipped = (torch.empty((), dtype=torch.float32, device=dev) for _ in range(3))
@@ -397,7 +398,7 @@ class _PolicyLoss(torch.autograd.Function):
         x, labels = ctx.saved_tensors
         d, ctx.gradient = ctx.gradient, None
         fresh = d is not None  # else a second pass through the graph: the first one's gradient has been given away
-        with _guard(x.device):
+        with guard(x.device):
             up = dloss.float()
             if fresh:
                 ld = _grad_ld(x)

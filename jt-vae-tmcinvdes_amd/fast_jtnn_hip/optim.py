@@ -17,6 +17,7 @@ import numpy as np
 import torch
 
 from . import _capi as K
+from .losses import guard
 
 _E4M3 = torch.float8_e4m3fn
 _SCALED = ("exp_avg_scale", "exp_rms_scale")
@@ -109,7 +110,7 @@ class _Group:
         if [n if g is None else g.numel() for g, n in zip(grads, self.numels)] != self.numels:
             raise RuntimeError("AdamW: a gradient has another size than its parameter had when the optimizer was built")
         if not all([g is None or (g.dtype is self.dtype and g.is_contiguous()) for g in grads]):
-            grads = keep = [None if g is None else g.to(self.dtype).contiguous() for g in grads]
+            grads = keep = [None if g is None else g.detach().to(self.dtype).contiguous() for g in grads]
         self.grads[:] = [None if g is None else g.data_ptr() for g in grads]
         return have, keep
 
@@ -217,14 +218,14 @@ class AdamW(torch.optim.Optimizer):
             if g.master:
                 g.copy_master()
 
-    @torch.no_grad()
     def step(self, closure=None):
+        """One step of every parameter that has a gradient; returns what ``closure`` (which forms the gradients) does."""
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
         max_norm = 0.0 if self.max_norm is None else float(self._check_norm(self.max_norm))
-        with torch.cuda.device(self._bound[0].device):
+        with guard(self._bound[0].device):
             work, keep, args, changed = [], [], [], []
             for g, hyper in zip(self._bound, self.param_groups):
                 self._check_hyper(hyper)
