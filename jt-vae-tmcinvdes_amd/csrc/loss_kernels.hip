@@ -139,7 +139,7 @@ __device__ __forceinline__ void take(RowStat& st, const float* v) {
   st.m = m;
 }
 
-// PolicyRow: r = exp(lp - old), term = w (kl_coef k3 - min(r A, clip(r) A)), k3 = exp(ref - lp) - (ref - lp) - 1
+// A policy row: r = exp(lp - old), term = w (kl_coef k3 - min(r A, clip(r) A)), k3 = exp(ref - lp) - (ref - lp) - 1
 // (an unbiased, never negative estimate of the KL divergence from the sampled label alone), and
 // d term / d lp = w (kl_coef (1 - exp(ref - lp)) - [r A <= clip(r) A] r A).
 struct PolicyRow {
@@ -198,8 +198,7 @@ __device__ __forceinline__ bool counts(const RowsIn<T>& in, int row, long label)
   return label >= 0 && !(in.owner && in.owner[row] < 0);
 }
 
-// Statistics of one long row per block, streamed: four 16-byte loads in flight per lane.  Reads at the rate of the
-// memory; a row of any length.
+// Statistics of one long row per block, streamed: four 16-byte loads in flight per lane; a row of any length.
 template <typename T, int BLOCK>
 __global__ __launch_bounds__(BLOCK) void stats_kernel(RowsIn<T> in) {
   constexpr int E = Vec<T>::E, U = 4;
@@ -266,16 +265,18 @@ enum { kStats = 0, kPolicy = 1 };
 // Whole rows in registers: RT lanes hold NV vectors of 16 bytes each, so a row is read once whatever is made of it.
 // kStats: statistics and log-probabilities of short rows.  kPolicy: the row's loss terms and, the coefficient of a policy
 // row depending on nothing else, its gradient in the same pass.  A block of RT * R threads owns R rows; the 64-bit
-// arithmetic of a row's end is done by one lane per row, side by side.
+// arithmetic of a row's end is done by one lane per row, side by side.  Bound by memory: 8192 x 32000 bf16 185 us in 512
+// threads x 8 vectors, 5.4 TB/s read and written (256 x 16 the same, 1024 x 4 199); 4096 x 128000 bf16, where a row
+// takes the registers of a CU and loads and stores do not overlap, 428 us, 4.9 TB/s - the two passes take 538.
 template <typename T, int RT, int R, int NV, int MODE>
-__global__ __launch_bounds__(RT* R, NV > 8 ? 4 : RT == 64 && NV == 8 ? 6 : 8) void rows_kernel(RowsIn<T> in, PolicyIn policy, float* __restrict__ coef,
-                                                     double* __restrict__ terms, long n_terms, GradOut<T> out) {
+__global__ __launch_bounds__(RT* R, NV > 8 ? 4 : RT == 64 && NV == 8 ? 6 : 8) void rows_kernel(
+    RowsIn<T> in, PolicyIn policy, float* __restrict__ coef, double* __restrict__ terms, long n_terms, GradOut<T> out) {
   constexpr int E = Vec<T>::E, W = RT / 64;
   // long policy rows are read once and for all: past the caches (8192 x 32000 bf16 201 -> 191 us); short ones lose by it
   // (20480 x 780 fp32 36 -> 40 us)
   constexpr bool kOnce = MODE == kPolicy && RT > 64;
   __shared__ RowStat part[R * W];
-  __shared__ float4 end[R];  // m, s, coefficient, counted
+  __shared__ float4 end[R];  // m, s, coefficient
   const int r = threadIdx.x / RT, t = threadIdx.x % RT;
   const long first = in.first + (long)blockIdx.x * R;
   const int row = (int)(first + r);
@@ -378,7 +379,11 @@ __global__ __launch_bounds__(RT* R, NV > 8 ? 4 : RT == 64 && NV == 8 ? 6 : 8) vo
 // dx[row, j] = c ([j = label] - exp(x_j - m) / s), c = coef[owner or row] * upstream, from saved statistics.  Rows are
 // cut into tiles of RT lanes x NV vectors; a block of 256 threads owns 256 / RT tiles.  With unless_one the gradient
 // for an upstream factor of one is in place already and nothing is done where the factor is one.
-template <typename T, int RT, int NV, bool ONCE>
+// Bound by memory: 4096 x 128000 bf16 341 us, 6.15 TB/s read and written.  Tiles of 8 KiB (two vectors a lane) keep the
+// places the chip works on close together: 8192 x 32000 bf16 169 us, with 16 KiB 188, with 4 KiB 209.  The gradient is
+// written past the caches, which leaves them to the logits: 60000 x 1500 fp32 125 us, through them 135; both passes of
+// 8192 x 32000 bf16 256 us instead of 305.
+template <typename T, int RT, int NV>
 __global__ __launch_bounds__(JTVAE_BLOCK) void grad_kernel(RowsIn<T> in, const float* __restrict__ coef,
                                                            const float* __restrict__ upstream, int unless_one,
                                                            int tiles, GradOut<T> out, float* __restrict__ scaled,
@@ -407,8 +412,7 @@ __global__ __launch_bounds__(JTVAE_BLOCK) void grad_kernel(RowsIn<T> in, const f
     if (counted) {
 #pragma unroll
       for (int u = 0; u < NV; ++u)
-        if (first + u * RT < n_vec)
-          w[u] = ONCE ? Vec<T>::load_once(x + shape.col(first + u * RT)) : Vec<T>::load(x + shape.col(first + u * RT));
+        if (first + u * RT < n_vec) w[u] = Vec<T>::load(x + shape.col(first + u * RT));
       const float2 st = in.stats[row];
       k = label < in.n_cols ? coef[own] * up : NAN;
       m = finite_or_zero(st.x);
@@ -466,7 +470,8 @@ __global__ __launch_bounds__(JTVAE_BLOCK) void sequence_sums_kernel(Sequences q,
                                                                     double* __restrict__ sums64,
                                                                     float* __restrict__ sums) {
   const int lane = threadIdx.x & 63;
-  for (long seq = ((long)blockIdx.x * JTVAE_BLOCK + threadIdx.x) >> 6; seq < q.n_seq; seq += (long)gridDim.x * (JTVAE_BLOCK / 64)) {
+  const long step = (long)gridDim.x * (JTVAE_BLOCK / 64);
+  for (long seq = ((long)blockIdx.x * JTVAE_BLOCK + threadIdx.x) >> 6; seq < q.n_seq; seq += step) {
     const double acc = sequence_sum(q, lp64, other, (int)seq, lane);
     if (lane == 0) {
       if (sums64) sums64[seq] = acc;
@@ -651,9 +656,11 @@ int launch_stats(const RowsIn<T>& rows, hipStream_t s) {
   });
 }
 
-// Statistics.  Rows of up to 512 vectors (8 KiB) sit in a wave's registers, eight waves side by side; longer ones are
-// streamed by a block each: 256 threads where there are rows enough to fill the chip with them, 1024 where there are
-// not (a row of 128 000 bf16 then has all its loads in flight on one CU).
+// Statistics.  Rows of up to 512 vectors (8 KiB) sit in a wave's registers, eight waves side by side (60000 x 1500 fp32
+// 58 us, 97 when streamed); longer ones are streamed by a block each.  Up to a row per CU the block has 512 threads, since
+// a CU alone is bound by its arithmetic (64 x 128000 bf16 10.7 us against 14.3, 256 rows 12.9 against 15.6); beyond, 256,
+// so that a CU has blocks at every stage (1024 x 30000 12.9 against 13.9, with 1024 threads 16.3).  Bound by memory from
+// there on: 4096 x 128000 bf16 178 us, 5.9 TB/s read.
 template <typename T>
 int row_stats(const jtvae_logits_t* g, const int32_t* owner, float* stats, float* lp32, double* lp64, hipStream_t s) {
   const RowsIn<T> in = rows_in<T>(g, owner, stats, lp32, lp64);
@@ -662,13 +669,13 @@ int row_stats(const jtvae_logits_t* g, const int32_t* owner, float* stats, float
   const GradOut<T> no_grad = {};
   if (n_vec <= 128) return launch_rows<T, 64, 8, 2, kStats>(in, none, nullptr, nullptr, no_grad, s);
   if (n_vec <= 512) return launch_rows<T, 64, 8, 8, kStats>(in, none, nullptr, nullptr, no_grad, s);
-  return g->n_rows >= 1024 ? launch_stats<T, 256>(in, s) : launch_stats<T, 1024>(in, s);
+  return g->n_rows > 256 ? launch_stats<T, 256>(in, s) : launch_stats<T, 512>(in, s);
 }
 
 // The grid where the gradient mostly stands already: enough to fill the chip once.
 constexpr unsigned kIdleBlocks = 2048;
 
-template <typename T, int RT, int NV, bool ONCE>
+template <typename T, int RT, int NV>
 int launch_grad(const RowsIn<T>& rows, const float* coef, const float* upstream, int unless_one, const GradOut<T>& out,
                 float* scaled, int n_scaled, hipStream_t s) {
   const int n_vec = rows.n_cols / Vec<T>::E;
@@ -676,7 +683,7 @@ int launch_grad(const RowsIn<T>& rows, const float* coef, const float* upstream,
   const auto launch = [&](const RowsIn<T>& in, int n) {
     unsigned blocks = n ? blocks_for((long)n * tiles, JTVAE_BLOCK / RT) : 1;
     if (unless_one && blocks > kIdleBlocks) blocks = kIdleBlocks;
-    hipLaunchKernelGGL((grad_kernel<T, RT, NV, ONCE>), dim3(blocks), dim3(JTVAE_BLOCK), 0, s, in, coef, upstream,
+    hipLaunchKernelGGL((grad_kernel<T, RT, NV>), dim3(blocks), dim3(JTVAE_BLOCK), 0, s, in, coef, upstream,
                        unless_one, tiles, out, scaled, n_scaled);
     n_scaled = 0;  // once is enough
   };
@@ -692,16 +699,14 @@ int row_grad(const jtvae_logits_t* g, const int32_t* owner, const float* stats, 
   const RowsIn<T> in = rows_in<T>(g, owner, (float*)stats, nullptr, nullptr);
   const GradOut<T> out = {(T*)dx, (long)ld_dx, (long)width};
   const int n_vec = g->n_cols / Vec<T>::E;
-  if (n_vec <= 128) return launch_grad<T, 64, 2, false>(in, coef, upstream, unless_one, out, scaled, n_scaled, s);
-  if (n_vec <= 256) return launch_grad<T, 64, 4, false>(in, coef, upstream, unless_one, out, scaled, n_scaled, s);
-  // Logits beyond what the 256 MiB cache keeps pass through it without staying: 4096 x 128000 bf16 397 -> 373 us,
-  // 2048 x 50000 fp32 141 -> 135 us; small ones must not (64 x 30000 bf16 5.4 -> 6.7 us).
-  if ((double)g->n_rows * g->n_cols * sizeof(T) > 128e6)
-    return launch_grad<T, 256, 2, true>(in, coef, upstream, unless_one, out, scaled, n_scaled, s);
-  return launch_grad<T, 256, 2, false>(in, coef, upstream, unless_one, out, scaled, n_scaled, s);
+  if (n_vec <= 128) return launch_grad<T, 64, 2>(in, coef, upstream, unless_one, out, scaled, n_scaled, s);
+  if (n_vec <= 256) return launch_grad<T, 64, 4>(in, coef, upstream, unless_one, out, scaled, n_scaled, s);
+  return launch_grad<T, 256, 2>(in, coef, upstream, unless_one, out, scaled, n_scaled, s);
 }
 
-// A policy row in one pass where its registers hold it; 1 when they do not.
+constexpr int kTooLong = -100;  // no error code of this library or of HIP
+
+// A policy row in one pass where its registers hold it; kTooLong when they do not.
 template <typename T>
 int policy_rows(const RowsIn<T>& in, const PolicyIn& p, float* coef, double* terms, const GradOut<T>& out,
                 hipStream_t s) {
@@ -712,7 +717,7 @@ int policy_rows(const RowsIn<T>& in, const PolicyIn& p, float* coef, double* ter
   if (n_vec <= 4096) return launch_rows<T, 512, 1, 8, kPolicy>(in, p, coef, terms, out, s);
   if (n_vec <= 8192) return launch_rows<T, 1024, 1, 8, kPolicy>(in, p, coef, terms, out, s);
   if (n_vec <= 16384) return launch_rows<T, 1024, 1, 16, kPolicy>(in, p, coef, terms, out, s);
-  return 1;
+  return kTooLong;
 }
 
 template <typename T>
@@ -720,7 +725,7 @@ int policy(const jtvae_logits_t* g, const PolicyIn& in, float* stats, float* lp,
            double* terms, void* dx, int64_t ld_dx, int64_t width, hipStream_t s) {
   const GradOut<T> out = {(T*)dx, (long)ld_dx, (long)width};
   const int rc = policy_rows<T>(rows_in<T>(g, nullptr, stats, lp, nullptr), in, coef, terms, out, s);
-  if (rc != 1) return rc;
+  if (rc != kTooLong) return rc;
   int e = row_stats<T>(g, nullptr, stats, lp, lp64, s);
   if (e) return e;
   hipLaunchKernelGGL(policy_rows_kernel, dim3(grid_for(g->n_rows)), dim3(JTVAE_BLOCK), 0, s, in, lp64,
@@ -811,9 +816,9 @@ int jtvae_preference_loss(const jtvae_logits_t* logits, const jtvae_sequences_t*
   const Preference in = {preference->ref_log_probs, preference->other_log_probs, preference->beta,
                          preference->label_smoothing, preference->scale};
   JT_CHECK(jtvae_label_log_probs(logits, sequences->row_seq, stats, nullptr, lp64, stream));
-  // Up to 64 sequences the one block of the pairs forms their sums as well, four per wave, and a launch is saved;
-  // beyond, a wave each (1024 sequences of 20 rows: 3.5 us, against 60 dependent gathers a wave).
-  if (n_seq <= 64) {
+  // For a few short sequences the one block of the pairs forms their sums as well, and a launch is saved (16 of 20 rows:
+  // 7.6 us instead of 10.1); else a wave each (64 of 300 rows: 15.8 us instead of 25.4, 1024 of 20: 14.8 instead of 66).
+  if (n_seq <= 64 && n <= 4096) {
     hipLaunchKernelGGL(preference_kernel<true>, dim3(1), dim3(kPairBlock), 0, s, q, in, lp64, sums64, sums, loss,
                        margins, dmargin, coef);
     return launch_status();
