@@ -383,7 +383,7 @@ __global__ __launch_bounds__(RT* R, NV > 8 ? 4 : RT == 64 && NV == 8 ? 6 : 8) vo
 // places the chip works on close together: 8192 x 32000 bf16 169 us, with 16 KiB 188, with 4 KiB 209.  The gradient is
 // written past the caches, which leaves them to the logits: 60000 x 1500 fp32 125 us, through them 135; both passes of
 // 8192 x 32000 bf16 256 us instead of 305.
-template <typename T, int RT, int NV>
+template <typename T, int RT, int NV, bool ONCE>
 __global__ __launch_bounds__(JTVAE_BLOCK) void grad_kernel(RowsIn<T> in, const float* __restrict__ coef,
                                                            const float* __restrict__ upstream, int unless_one,
                                                            int tiles, GradOut<T> out, float* __restrict__ scaled,
@@ -412,7 +412,8 @@ __global__ __launch_bounds__(JTVAE_BLOCK) void grad_kernel(RowsIn<T> in, const f
     if (counted) {
 #pragma unroll
       for (int u = 0; u < NV; ++u)
-        if (first + u * RT < n_vec) w[u] = Vec<T>::load(x + shape.col(first + u * RT));
+        if (first + u * RT < n_vec)
+          w[u] = ONCE ? Vec<T>::load_once(x + shape.col(first + u * RT)) : Vec<T>::load(x + shape.col(first + u * RT));
       const float2 st = in.stats[row];
       k = label < in.n_cols ? coef[own] * up : NAN;
       m = finite_or_zero(st.x);
@@ -675,7 +676,7 @@ int row_stats(const jtvae_logits_t* g, const int32_t* owner, float* stats, float
 // The grid where the gradient mostly stands already: enough to fill the chip once.
 constexpr unsigned kIdleBlocks = 2048;
 
-template <typename T, int RT, int NV>
+template <typename T, int RT, int NV, bool ONCE>
 int launch_grad(const RowsIn<T>& rows, const float* coef, const float* upstream, int unless_one, const GradOut<T>& out,
                 float* scaled, int n_scaled, hipStream_t s) {
   const int n_vec = rows.n_cols / Vec<T>::E;
@@ -683,7 +684,7 @@ int launch_grad(const RowsIn<T>& rows, const float* coef, const float* upstream,
   const auto launch = [&](const RowsIn<T>& in, int n) {
     unsigned blocks = n ? blocks_for((long)n * tiles, JTVAE_BLOCK / RT) : 1;
     if (unless_one && blocks > kIdleBlocks) blocks = kIdleBlocks;
-    hipLaunchKernelGGL((grad_kernel<T, RT, NV>), dim3(blocks), dim3(JTVAE_BLOCK), 0, s, in, coef, upstream,
+    hipLaunchKernelGGL((grad_kernel<T, RT, NV, ONCE>), dim3(blocks), dim3(JTVAE_BLOCK), 0, s, in, coef, upstream,
                        unless_one, tiles, out, scaled, n_scaled);
     n_scaled = 0;  // once is enough
   };
@@ -699,9 +700,13 @@ int row_grad(const jtvae_logits_t* g, const int32_t* owner, const float* stats, 
   const RowsIn<T> in = rows_in<T>(g, owner, (float*)stats, nullptr, nullptr);
   const GradOut<T> out = {(T*)dx, (long)ld_dx, (long)width};
   const int n_vec = g->n_cols / Vec<T>::E;
-  if (n_vec <= 128) return launch_grad<T, 64, 2>(in, coef, upstream, unless_one, out, scaled, n_scaled, s);
-  if (n_vec <= 256) return launch_grad<T, 64, 4>(in, coef, upstream, unless_one, out, scaled, n_scaled, s);
-  return launch_grad<T, 256, 2>(in, coef, upstream, unless_one, out, scaled, n_scaled, s);
+  if (n_vec <= 128) return launch_grad<T, 64, 2, false>(in, coef, upstream, unless_one, out, scaled, n_scaled, s);
+  if (n_vec <= 256) return launch_grad<T, 64, 4, false>(in, coef, upstream, unless_one, out, scaled, n_scaled, s);
+  // Logits beyond what the 256 MiB cache keeps are read past it (forward and backward of 4096 x 128000 bf16: 482 us, 493
+  // through it); smaller ones are found there (4000 x 3500 bf16 11.0 us, 12.7 past it).
+  if ((double)g->n_rows * g->n_cols * sizeof(T) > 256e6)
+    return launch_grad<T, 256, 2, true>(in, coef, upstream, unless_one, out, scaled, n_scaled, s);
+  return launch_grad<T, 256, 2, false>(in, coef, upstream, unless_one, out, scaled, n_scaled, s);
 }
 
 constexpr int kTooLong = -100;  // no error code of this library or of HIP

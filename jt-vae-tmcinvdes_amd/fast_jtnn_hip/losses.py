@@ -181,6 +181,10 @@ def guard(device):
     return _NOTHING if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
+def _wants_grad(t):
+    return t.requires_grad and torch.is_grad_enabled()
+
+
 def _rows(logits):
     """The logits themselves, or a copy where columns are strided or rows overlap."""
     (n, v), (s0, s1) = logits.shape, logits.stride()
@@ -197,28 +201,14 @@ def _arg(x, labels):
                     64 if labels.dtype is torch.int64 else 32), labels
 
 
-def _again(ctx, x, labels):
-    """The backward pass's jtvae_logits_t: the forward's, unless the saved tensors came back at another place."""
-    g, keep = ctx.arg
-    if x.data_ptr() != g.x or labels.data_ptr() != g.labels:
-        ctx.arg = g, keep = _arg(x, labels)
-    return g
-
-
 def _grad_rows(x):
     """(uninitialised gradient in the layout of ``x``, its leading dimension): the few padding columns of the package's
     row buffers are kept - the kernel writes them as zero - so that the products that follow take it without a copy."""
     n, v = x.shape
-    ld = _grad_ld(x)
-    if ld == v:
-        return torch.empty((n, v), dtype=x.dtype, device=x.device), ld
-    return torch.empty((n, ld), dtype=x.dtype, device=x.device)[:, :v], ld
-
-
-def _grad_ld(x):
-    n, v = x.shape
     ld = x.stride(0) if n > 1 else v
-    return ld if v <= ld < v + 64 else v
+    if not v < ld < v + 64:
+        return torch.empty((n, v), dtype=x.dtype, device=x.device), v
+    return torch.empty((n, ld), dtype=x.dtype, device=x.device)[:, :v], ld
 
 
 def _scratch(device, *counts):
@@ -231,15 +221,47 @@ def _scratch(device, *counts):
     return buf, out
 
 
+class _Gradient:
+    """The gradient of a call's logits.  What can be made ready is made with the forward pass: autograd runs the backward
+    pass on a thread of its own, which has just been woken and takes two to three times as long over the same Python.
+    Buffers of up to ``EARLY_BYTES`` are among it (24 x 385, both passes: 112 -> 90 us on one machine); larger ones
+    are not held between the passes."""
+
+    EARLY_BYTES = 4 << 20
+
+    __slots__ = ("g", "keep", "x_at", "y_at", "buffer", "ld", "made")
+
+    def __init__(self, x, labels, g, keep, want, made=False):
+        """``made``: the buffer will hold the gradient for an upstream factor of one when the forward pass ends."""
+        self.g, self.keep, self.x_at, self.y_at, self.buffer, self.made = g, keep, x.data_ptr(), labels.data_ptr(), None, made
+        if want and (made or g.n_rows * g.n_cols * x.element_size() <= self.EARLY_BYTES):
+            self.buffer, self.ld = _grad_rows(x)
+
+    def __call__(self, x, labels, owner, stats, coef, up, scaled=None, n_scaled=0):
+        """The gradient from saved statistics and coefficients (addresses), on the device and stream of the forward pass,
+        which autograd has made the current ones."""
+        d, self.buffer = self.buffer, None
+        unless_one = self.made and d is not None
+        if d is None:  # not held, or given away by an earlier pass through the same graph
+            d, self.ld = _grad_rows(x)
+        if x.data_ptr() != self.x_at or labels.data_ptr() != self.y_at:  # saved tensors may come back at another place
+            self.g, self.keep = _arg(x, labels)
+            self.x_at, self.y_at = x.data_ptr(), labels.data_ptr()
+        K.label_log_probs_bwd(self.g, owner, stats, coef, up, d.data_ptr(), self.ld, self.ld, int(unless_one), scaled,
+                              n_scaled)
+        return d
+
+
 class _TokenLogProbs(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, labels):
+    def forward(ctx, logits, labels, want):
         x, dev, n = _rows(logits), logits.device, logits.shape[0]
         with guard(dev):
             lp = torch.empty((n,), dtype=torch.float32, device=dev)
             ctx.ws, (stats,) = _scratch(dev, n)
-            ctx.arg = g, _ = _arg(x, labels)
+            g, keep = _arg(x, labels)
             K.label_log_probs(g, None, stats, lp.data_ptr(), None)
+            ctx.gradient = _Gradient(x, labels, g, keep, want)
         ctx.save_for_backward(x, labels)
         return lp
 
@@ -247,30 +269,28 @@ class _TokenLogProbs(torch.autograd.Function):
     @_differentiable_once
     def backward(ctx, dlp):
         x, labels = ctx.saved_tensors
-        with guard(x.device):
-            coef = dlp.float().contiguous()
-            d, ld = _grad_rows(x)
-            K.label_log_probs_bwd(_again(ctx, x, labels), None, ctx.ws.data_ptr(), coef.data_ptr(), None, d.data_ptr(), ld, ld)
-        return d, None
+        coef = dlp.contiguous()
+        return ctx.gradient(x, labels, None, ctx.ws.data_ptr(), coef.data_ptr(), None), None, None
 
 
 def token_log_probs(logits: torch.Tensor, labels: torch.Tensor) -> torch.Tensor:
     """[N] fp32: log softmax(logits[i])[labels[i]], 0 where the label is negative.  Differentiable in ``logits``."""
     _check("token_log_probs", logits, labels)
     _on_device("token_log_probs", logits, labels=labels)
-    return _TokenLogProbs.apply(logits, labels)
+    return _TokenLogProbs.apply(logits, labels, _wants_grad(logits))
 
 
 class _SequenceLogProbs(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, labels, plan):
+    def forward(ctx, logits, labels, plan, want):
         x, dev, n = _rows(logits), logits.device, logits.shape[0]
         with guard(dev):
             plan.on_current_stream()
             sums = torch.empty((plan.n_seq,), dtype=torch.float32, device=dev)
             ctx.ws, (stats, ws) = _scratch(dev, n, n)
-            ctx.arg = g, _ = _arg(x, labels)
+            g, keep = _arg(x, labels)
             K.sequence_log_probs(g, plan.arg, stats, sums.data_ptr(), ws, 8 * n)
+            ctx.gradient = _Gradient(x, labels, g, keep, want)
         ctx.save_for_backward(x, labels)
         ctx.plan = plan
         return sums
@@ -279,14 +299,9 @@ class _SequenceLogProbs(torch.autograd.Function):
     @_differentiable_once
     def backward(ctx, dsums):
         x, labels = ctx.saved_tensors
-        with guard(x.device):
-            coef = dsums.float().contiguous()
-            d, ld = _grad_rows(x)
-            g, keep = _arg(x, labels)
-            # without sequences no row counts and the coefficients are never read: any address will do
-            K.label_log_probs_bwd(g, ctx.plan.arg.row_seq, ctx.ws.data_ptr(), coef.data_ptr() or ctx.ws.data_ptr(), None,
-                                  d.data_ptr(), ld, ld)
-        return d, None, None
+        stats, coef = ctx.ws.data_ptr(), dsums.contiguous()
+        # without sequences no row counts and the coefficients are never read: any address will do
+        return ctx.gradient(x, labels, ctx.plan.arg.row_seq, stats, coef.data_ptr() or stats, None), None, None, None
 
 
 def sequence_log_probs(logits: torch.Tensor, labels: torch.Tensor, plan: SequencePlan) -> torch.Tensor:
@@ -295,12 +310,12 @@ def sequence_log_probs(logits: torch.Tensor, labels: torch.Tensor, plan: Sequenc
     _check("sequence_log_probs", logits, labels)
     _check_plan("sequence_log_probs", plan, logits)
     _on_device("sequence_log_probs", logits, labels=labels, plan=plan)
-    return _SequenceLogProbs.apply(logits, labels, plan)
+    return _SequenceLogProbs.apply(logits, labels, plan, _wants_grad(logits))
 
 
 class _PreferenceLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, other, labels, plan, ref, beta, smoothing, scale):
+    def forward(ctx, logits, other, labels, plan, ref, beta, smoothing, scale, want, want_other):
         x, dev, n, S, P = _rows(logits), logits.device, logits.shape[0], plan.n_seq, plan.n_pairs
         with guard(dev):
             plan.on_current_stream()
@@ -309,11 +324,13 @@ class _PreferenceLoss(torch.autograd.Function):
             margins = torch.empty((P,), dtype=torch.float32, device=dev)
             loss = torch.empty((), dtype=torch.float32, device=dev)
             ctx.ws, (stats, coef, ws) = _scratch(dev, n, (S + 1) // 2, n + S + P)
-            ctx.arg = g, _ = _arg(x, labels)
+            g, keep = _arg(x, labels)
             K.preference_loss(g, plan.arg, K.Preference(ref.data_ptr(), K.ptr(oth), beta, smoothing, scale), stats,
                               sums.data_ptr(), margins.data_ptr(), coef, loss.data_ptr(), ws, 8 * (n + S + P))
+            ctx.gradient = _Gradient(x, labels, g, keep, want)
+            ctx.dother = torch.empty((S,), dtype=torch.float32, device=dev) if want_other else None
         ctx.save_for_backward(x, labels)
-        ctx.plan, ctx.other_dtype = plan, None if other is None else other.dtype
+        ctx.plan, ctx.at, ctx.other_dtype = plan, (stats, coef), None if other is None else other.dtype
         ctx.mark_non_differentiable(sums, margins)
         ctx.set_materialize_grads(False)
         return loss, sums, margins
@@ -322,25 +339,22 @@ class _PreferenceLoss(torch.autograd.Function):
     @_differentiable_once
     def backward(ctx, dloss, *_):
         if dloss is None:
-            return (None,) * 8
+            return (None,) * 10
         x, labels = ctx.saved_tensors
-        plan, d, dother = ctx.plan, None, None
-        stats = ctx.ws.data_ptr()
-        coef = stats + 8 * x.shape[0]
-        with guard(x.device):
-            up = dloss.float()
-            if ctx.needs_input_grad[1]:
-                dother = torch.empty((plan.n_seq,), dtype=torch.float32, device=x.device)
-            if ctx.needs_input_grad[0]:
-                d, ld = _grad_rows(x)
-                K.label_log_probs_bwd(_again(ctx, x, labels), plan.arg.row_seq, stats, coef, up.data_ptr(), d.data_ptr(), ld, ld,
-                                      scaled=K.ptr(dother), n_scaled=0 if dother is None else plan.n_seq)
-            elif dother is not None:
-                at = 2 * x.shape[0]
-                torch.mul(ctx.ws.view(torch.float32)[at:at + plan.n_seq], up, out=dother)
-            if dother is not None and ctx.other_dtype is not torch.float32:
-                dother = dother.to(ctx.other_dtype)
-        return d, dother, None, None, None, None, None, None
+        plan, d, (stats, coef) = ctx.plan, None, ctx.at
+        want, want_other = ctx.needs_input_grad[:2]
+        dother, ctx.dother = ctx.dother, None
+        if want_other and dother is None:  # a second pass through the graph
+            dother = torch.empty((plan.n_seq,), dtype=torch.float32, device=x.device)
+        if want:
+            d = ctx.gradient(x, labels, plan.arg.row_seq, stats, coef, dloss.data_ptr(), K.ptr(dother),
+                             plan.n_seq if want_other else 0)
+        elif want_other:
+            at = 2 * x.shape[0]
+            torch.mul(ctx.ws.view(torch.float32)[at:at + plan.n_seq], dloss, out=dother)
+        if want_other and ctx.other_dtype is not torch.float32:
+            dother = dother.to(ctx.other_dtype)
+        return d, dother, None, None, None, None, None, None, None, None
 
 
 def preference_loss(logits: torch.Tensor, labels: torch.Tensor, plan: SequencePlan, ref_log_probs: torch.Tensor,
@@ -364,13 +378,14 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, plan: SequencePl
     smoothing = _number(what, "label_smoothing", label_smoothing, 0.0, 1.0)
     scale = 1.0 / max(plan.n_pairs, 1) if scale is None else _number(what, "scale", scale, -float("inf"))
     _on_device(what, logits, labels=labels, plan=plan, ref_log_probs=ref_log_probs, other_log_probs=other_log_probs)
-    return PreferenceLoss(*_PreferenceLoss.apply(logits, other_log_probs, labels, plan, ref_log_probs, beta, smoothing,
-                                                 scale))
+    return PreferenceLoss(*_PreferenceLoss.apply(
+        logits, other_log_probs, labels, plan, ref_log_probs, beta, smoothing, scale, _wants_grad(logits),
+        other_log_probs is not None and _wants_grad(other_log_probs)))
 
 
 class _PolicyLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, labels, old, adv, ref, weights, lo, hi, kl_coef, scale, want_grad):
+    def forward(ctx, logits, labels, old, adv, ref, weights, lo, hi, kl_coef, scale, want):
         x, dev, n = _rows(logits), logits.device, logits.shape[0]
         with guard(dev):
             old, adv, ref, weights = (_fp32(t) for t in (old, adv, ref, weights))
@@ -378,14 +393,15 @@ class _PolicyLoss(torch.autograd.Function):
             loss, kl, clipped = (torch.empty((), dtype=torch.float32, device=dev) for _ in range(3))
             nbytes = K.policy_loss_workspace_bytes(n)
             ctx.ws, (stats, coef, ws) = _scratch(dev, n, (n + 1) // 2, nbytes // 8)
+            g, keep = _arg(x, labels)
             # a row's coefficient depends on that row alone: its gradient is made while the row is in registers
-            d, ld = _grad_rows(x) if want_grad else (None, 0)
-            ctx.arg = g, _ = _arg(x, labels)
+            ctx.gradient = made = _Gradient(x, labels, g, keep, want, made=True)
+            ld = made.ld if want else 0
             policy = K.Policy(old.data_ptr(), adv.data_ptr(), K.ptr(ref), K.ptr(weights), lo, hi, kl_coef, scale)
             K.policy_loss(g, policy, stats, lp.data_ptr(), coef, loss.data_ptr(), kl.data_ptr(), clipped.data_ptr(),
-                          K.ptr(d), ld, ld, ws, nbytes)
+                          K.ptr(made.buffer), ld, ld, ws, nbytes)
         ctx.save_for_backward(x, labels)
-        ctx.gradient = d
+        ctx.at = stats, coef
         ctx.mark_non_differentiable(lp, kl, clipped)
         ctx.set_materialize_grads(False)
         return loss, lp, kl, clipped
@@ -396,19 +412,8 @@ class _PolicyLoss(torch.autograd.Function):
         if dloss is None:
             return (None,) * 11
         x, labels = ctx.saved_tensors
-        d, ctx.gradient = ctx.gradient, None
-        fresh = d is not None  # else a second pass through the graph: the first one's gradient has been given away
-        with guard(x.device):
-            up = dloss.float()
-            if fresh:
-                ld = _grad_ld(x)
-            else:
-                d, ld = _grad_rows(x)
-            stats = ctx.ws.data_ptr()
-            # a fresh gradient stands as it is where the upstream factor is 1, which only the device knows
-            K.label_log_probs_bwd(_again(ctx, x, labels), None, stats, stats + 8 * x.shape[0], up.data_ptr(), d.data_ptr(), ld, ld,
-                                  unless_one=int(fresh))
-        return (d,) + (None,) * 10
+        # a fresh gradient stands as it is where the upstream factor is 1, which only the device knows
+        return (ctx.gradient(x, labels, None, *ctx.at, dloss.data_ptr()),) + (None,) * 10
 
 
 def policy_loss(logits: torch.Tensor, labels: torch.Tensor, old_log_probs: torch.Tensor, advantages: torch.Tensor,
@@ -437,4 +442,4 @@ def policy_loss(logits: torch.Tensor, labels: torch.Tensor, old_log_probs: torch
         raise ValueError("%s: kl_coef needs ref_log_probs" % what)
     _on_device(what, logits, labels=labels, **given)
     return PolicyLoss(*_PolicyLoss.apply(logits, labels, old_log_probs, advantages, ref_log_probs, weights, lo, hi,
-                                         kl_coef, scale, logits.requires_grad and torch.is_grad_enabled()))
+                                         kl_coef, scale, _wants_grad(logits)))
