@@ -103,16 +103,19 @@ class _Group:
 
     def gather_grads(self):
         """Fills the address list; (parameters with a gradient, tensors to keep alive until the launches)."""
-        grads, have, keep = [p.grad for p in self.params], self.params, []
-        missing = [g is None for g in grads]
-        if any(missing):
-            have = [p for p, m in zip(self.params, missing) if not m]
-        if [n if g is None else g.numel() for g, n in zip(grads, self.numels)] != self.numels:
+        grads, dt = [p.grad for p in self.params], self.dtype
+        try:  # the usual case in three passes without a branch: every parameter has a plain gradient
+            plain = [g.numel() for g in grads] == self.numels and all([g.dtype is dt and g.is_contiguous() for g in grads])
+        except AttributeError:
+            plain = False
+        if plain:
+            self.grads[:] = [g.data_ptr() for g in grads]
+            return self.params, grads
+        if any(g is not None and g.numel() != n for g, n in zip(grads, self.numels)):
             raise RuntimeError("AdamW: a gradient has another size than its parameter had when the optimizer was built")
-        if not all([g is None or (g.dtype is self.dtype and g.is_contiguous()) for g in grads]):
-            grads = keep = [None if g is None else g.detach().to(self.dtype).contiguous() for g in grads]
+        grads = [None if g is None else g.detach().to(dt).contiguous() for g in grads]
         self.grads[:] = [None if g is None else g.data_ptr() for g in grads]
-        return have, keep
+        return [p for p, g in zip(self.params, grads) if g is not None], grads
 
     def args(self, hyper):
         lr = hyper["lr"]
