@@ -620,6 +620,7 @@ typedef struct jtvae_adamw_group {
   int32_t dtype;               /* JTVAE_F32 / F16 / BF16                                               */
   int32_t state_bits;          /* 32 or 8                                                              */
   int32_t use_master;          /* 16-bit parameters: the step works on the tensors' master copies      */
+  int32_t stochastic;          /* 8-bit states: rounded at random with the right mean, not to nearest  */
   const float* lr_device;      /* device scalar that replaces lr, or NULL                              */
   double lr, beta1, beta2, eps, weight_decay;
 } jtvae_adamw_group_t;
@@ -630,7 +631,8 @@ typedef struct jtvae_adamw_group {
  *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
  *   w = w (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
  * on the fp32 copy where there is one, whose rounded value then becomes the parameter.  8-bit states hold m and
- * sqrt(v) as e4m3 values times the block's scale max / 448, rounded to nearest after the update; a root that is not
+ * sqrt(v) as e4m3 values times the block's scale max / 448, rounded after the update: to nearest, or (stochastic) to one
+ * of the two neighbours, by bits that are a function of element, tensor and step alone; a root that is not
  * zero keeps at least the smallest value 2^-9, so that it never leaves m divided by eps alone.  A maximum of at most
  * 2^-100 counts as zero.  An element that is not finite becomes NaN and leaves the rest of its block as it is. */
 int jtvae_adamw_step(const jtvae_adamw_group_t* groups, int32_t n_groups, double max_norm, double* partials,

@@ -166,6 +166,7 @@ __global__ __launch_bounds__(kPrepBlock) void prepare_kernel(int* __restrict__ s
 struct Hyper {
   float lr, decay, beta1, one_m_beta1, beta2, one_m_beta2, eps;
   const float *lr_device, *grad_scale;
+  const int* steps;  // where rounding is stochastic, else NULL
 };
 
 // The four e4m3 values of a word, and back with the format's rounding to nearest even.
@@ -195,14 +196,32 @@ __device__ __forceinline__ float block_top(const float v[4]) {
   return t;
 }
 
+// Well mixed bits of a counter (xor-shifts and odd multipliers; every output once over all counters).
+__device__ __forceinline__ unsigned mix(unsigned x) {
+  x = (x ^ (x >> 16)) * 0x7feb352du;
+  x = (x ^ (x >> 15)) * 0x846ca68bu;
+  return x ^ (x >> 16);
+}
+
+// One of the two e4m3 values next to x (|x| <= 448), the nearer the likelier, so that the mean is x: the bits below the
+// format's last place are added to and cut off.  Below 2^-6 the format's places are as wide as between 2^-6 and 2^-5,
+// where the value is shifted for it.
+__device__ __forceinline__ float round_by(float x, unsigned bits20) {
+  const float a = fabsf(x), low = a < 0x1p-6f ? 0x1p-6f : 0.f;
+  const unsigned w = (__float_as_uint(a + low) + bits20) & 0xfff00000u;
+  return copysignf(fminf(__uint_as_float(w) - low, kTop), x);
+}
+
+// e4m3 values of v over the block's scale.  `dice`: 0 = to nearest, else 20 random bits per element (low 20 bits of each).
 template <bool ROOT>
-__device__ __forceinline__ unsigned quantise(const float v[4], float top) {
+__device__ __forceinline__ unsigned quantise(const float v[4], float top, bool by_dice, const unsigned dice[4]) {
   const float inv = top > kSmallest ? kTop / top : 0.f;
   float x[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     float y = fminf(fmaxf(v[k] * inv, -kTop), kTop);
-    if (ROOT) y = y > 0.f ? fmaxf(y, 0x1p-9f) : y;
+    if (by_dice) y = round_by(y, dice[k]);
+    if (ROOT) y = v[k] > 0.f && inv > 0.f ? fmaxf(y, 0x1p-9f) : y;
     x[k] = fabsf(v[k]) < INFINITY ? y : NAN;
   }
   return pack_e4m3(x);
@@ -216,6 +235,7 @@ __device__ __forceinline__ float root(float v) {
 }
 
 struct Step {
+  unsigned dice;  // of the tensor and its step; 0: round to nearest
   float keep, rate, eps, beta1, one_m_beta1, beta2, one_m_beta2, grad_scale, bias2;
 };
 
@@ -266,8 +286,17 @@ __device__ __forceinline__ void update(const jtvae_adamw_tensor_t& t, const T* g
         if (at + k >= t.n) m[k] = r[k] = 0.f;
     }
     const float tm = block_top(m), tr = block_top(r);
-    __builtin_nontemporal_store(quantise<false>(m, tm), (unsigned*)((uint8_t*)t.exp_avg + at));
-    __builtin_nontemporal_store(quantise<true>(r, tr), (unsigned*)((uint8_t*)t.second + at));
+    unsigned dm[4], dr[4];
+    if (s.dice) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const unsigned x = mix((unsigned)(at + k) ^ s.dice ^ (unsigned)((at + k) >> 32) * 0x9e3779b9u);
+        dm[k] = x >> 12;
+        dr[k] = mix(x) >> 12;
+      }
+    }
+    __builtin_nontemporal_store(quantise<false>(m, tm, s.dice != 0, dm), (unsigned*)((uint8_t*)t.exp_avg + at));
+    __builtin_nontemporal_store(quantise<true>(r, tr, s.dice != 0, dr), (unsigned*)((uint8_t*)t.second + at));
     if ((threadIdx.x & 63) == 0) {
       t.exp_avg_scale[at / kGroup] = tm > kSmallest ? tm / kTop : 0.f;
       t.second_scale[at / kGroup] = tr > kSmallest ? tr / kTop : 0.f;
@@ -296,7 +325,9 @@ __global__ __launch_bounds__(kBlock) void adamw_kernel(const jtvae_adamw_tensor_
   if (at / kGroup * kGroup >= t.n) return;  // the same for the lanes of a wave: the first element of their block
   const float2 b = bias[c.x];
   const float lr = h.lr_device ? *h.lr_device : h.lr;
-  const Step s = {1.f - lr * h.decay, lr * b.x,      h.eps, h.beta1, h.one_m_beta1, h.beta2, h.one_m_beta2,
+  // the same rounding for the same step of the same tensor, whatever the launch
+  const unsigned dice = BITS == 8 && h.steps ? mix((unsigned)h.steps[c.x] * 0x9e3779b9u + (unsigned)c.x) | 1u : 0u;
+  const Step s = {dice, 1.f - lr * h.decay, lr * b.x,      h.eps, h.beta1, h.one_m_beta1, h.beta2, h.one_m_beta2,
                   h.grad_scale ? *h.grad_scale : 1.f, b.y};
   if (base + kRound <= t.n) update<T, MASTER, BITS, true>(t, g, s, at);
   else update<T, MASTER, BITS, false>(t, g, s, at);
@@ -408,7 +439,8 @@ int jtvae_adamw_step(const jtvae_adamw_group_t* groups, int32_t n_groups, double
     const jtvae_adamw_group_t& g = groups[i];
     const Hyper h = {(float)g.lr,    (float)g.weight_decay,  (float)g.beta1, (float)(1.0 - g.beta1),
                      (float)g.beta2, (float)(1.0 - g.beta2), (float)g.eps,   g.lr_device,
-                     max_norm > 0.0 ? norm + 1 : nullptr};
+                     max_norm > 0.0 ? norm + 1 : nullptr,
+                     g.stochastic ? g.steps : nullptr};
     const bool master = g.dtype != JTVAE_F32 && g.use_master;
     int rc;
     switch (g.dtype) {

@@ -210,7 +210,7 @@ class AdamwTensor(C.Structure):  # jtvae_adamw_tensor_t
 class AdamwGroup(C.Structure):  # jtvae_adamw_group_t
     _fields_ = ([(n, C.c_void_p) for n in ("tensors", "chunks", "chunk_ptr", "grads", "steps", "bias")] +
                 [("n_tensors", C.c_int32), ("n_chunks", C.c_int64), ("dtype", C.c_int32), ("state_bits", C.c_int32),
-                 ("use_master", C.c_int32), ("lr_device", C.c_void_p)] +
+                 ("use_master", C.c_int32), ("stochastic", C.c_int32), ("lr_device", C.c_void_p)] +
                 [(n, C.c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay")])
 
 

@@ -6,7 +6,11 @@ step is one launch per group whatever the number of tensors, two more if the gra
 
 States live in one buffer per group and kind; ``optimizer.state[p]`` holds views of them.  With ``state_bits=8`` the
 first moment and the square root of the second are kept as e4m3 values with one fp32 scale per 256 elements: 2.03 bytes
-per parameter instead of 8.  16-bit parameters are stepped on an fp32 copy (``master=True``), since a step is usually
+per parameter instead of 8.  Such a value has three bits behind the point, and a step with ``beta2 = 0.999`` moves a root by
+less than half a place: rounded to nearest, an element's share in its block stands still until a gradient is eight to
+eleven times its root, and only the block's scale follows the gradients.  ``rounding="stochastic"`` rounds to one of the
+two neighbours with the right mean instead (by bits that are a function of element, tensor and step: runs repeat), so
+that every element follows its own gradients, within some 15 % of the root.  16-bit parameters are stepped on an fp32 copy (``master=True``), since a step is usually
 smaller than half their last place.
 """
 from __future__ import annotations
@@ -131,7 +135,7 @@ class _Group:
         return K.AdamwGroup(self.table.data_ptr(), self.chunks.data_ptr(), self.chunk_ptr.ctypes.data,
                             C.cast(self.grads, C.c_void_p), self.steps.data_ptr(), self.bias.data_ptr(),
                             len(self.params), self.n_chunks, K.DTYPE_CODE[self.dtype], self.bits, int(self.master),
-                            lr_dev, lr, b1, b2, hyper["eps"], hyper["weight_decay"])
+                            int(hyper["rounding"] == "stochastic"), lr_dev, lr, b1, b2, hyper["eps"], hyper["weight_decay"])
 
 
 class AdamW(torch.optim.Optimizer):
@@ -140,7 +144,7 @@ class AdamW(torch.optim.Optimizer):
         m = beta1 m + (1 - beta1) g,   v = beta2 v + (1 - beta2) g^2,
         w = w (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps).
 
-    ``state_bits``: 32, or 8 (see the module).  ``master``: 16-bit parameters keep an fp32 copy that the step works on; it
+    ``state_bits``: 32, or 8; ``rounding`` of 8-bit states: "nearest" or "stochastic" (see the module).  ``master``: 16-bit parameters keep an fp32 copy that the step works on; it
     is the optimizer's, so a value written into such a parameter from outside needs ``refresh_master()``.  ``max_norm``:
     gradients are multiplied by ``min(1, max_norm / (norm + 1e-6))``, norm being the 2-norm over all parameters of all
     groups - inside the step, ``.grad`` keeps what backward left; ``grad_norm`` (a 0-d device tensor) holds the norm of
@@ -149,12 +153,12 @@ class AdamW(torch.optim.Optimizer):
     between replays is a float32 tensor on the device."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, master=True,
-                 max_norm=None):
+                 max_norm=None, rounding="nearest"):
         self._bound = []
         self._norm = None
         self.max_norm = self._check_norm(max_norm)
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
-                                      master=master))
+                                      master=master, rounding=rounding))
 
     @staticmethod
     def _check_norm(max_norm):
@@ -171,6 +175,8 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("AdamW: betas = %r" % (g["betas"],))
         if not (g["eps"] >= 0 and g["weight_decay"] >= 0):
             raise ValueError("AdamW: eps = %r, weight_decay = %r" % (g["eps"], g["weight_decay"]))
+        if g["rounding"] not in ("nearest", "stochastic"):
+            raise ValueError("AdamW: rounding is nearest or stochastic, got %r" % (g["rounding"],))
 
     def add_param_group(self, param_group):
         super().add_param_group(param_group)

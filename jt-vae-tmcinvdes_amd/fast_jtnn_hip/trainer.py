@@ -77,8 +77,8 @@ class Trainer:
 
     def __init__(self, model: nn.Module, sched: Schedule = None, save_dir: str = None, conditional: bool = False,
                  total_step: int = 0, log=print, optimizer: str = "adam", weight_decay: float = 0.0):
-        """``optimizer``: "adam" (the reference's), or "adamw" / "adamw8", the package's AdamW with 32- or 8-bit states,
-        which clips inside its step: ``.grad`` then keeps the unclipped gradient."""
+        """``optimizer``: "adam" (the reference's), or "adamw" / "adamw8", the package's AdamW with 32- or 8-bit states
+        (the latter rounded stochastically), which clips inside its step: ``.grad`` then keeps the unclipped gradient."""
         if optimizer not in OPTIMIZERS:
             raise ValueError("optimizer %r is none of %s" % (optimizer, ", ".join(OPTIMIZERS)))
         if optimizer == "adam" and weight_decay:
@@ -91,7 +91,8 @@ class Trainer:
             from .optim import AdamW
 
             self.optimizer = AdamW(self.params, lr=self.sched.lr, weight_decay=weight_decay,
-                                   state_bits=8 if optimizer == "adamw8" else 32, max_norm=self.sched.clip_norm)
+                                   state_bits=8 if optimizer == "adamw8" else 32, max_norm=self.sched.clip_norm,
+                                   rounding="stochastic")
         else:
             self.optimizer = torch.optim.Adam(self.params, lr=self.sched.lr)  # vae_train.py:73-74
         self.scheduler = torch.optim.lr_scheduler.ExponentialLR(self.optimizer, self.sched.anneal_rate)

@@ -234,6 +234,75 @@ def test_extreme_gradients(bits):
         assert (st["exp_rms"].float()[512:600] > 0).all()  # far below the maximum, not zero
 
 
+def test_stochastic_rounding():
+    """Either neighbour of the exact value, the right one on average, the same in every run; zeros stay zero, roots that
+    are not zero stay above it, and what is not finite is marked."""
+    from fast_jtnn_hip import AdamW
+
+    n = 1 << 20
+    g = torch.Generator(device="cuda").manual_seed(3)
+    grad = torch.randn(n, generator=g, device="cuda") * torch.exp(torch.randn(n, generator=g, device="cuda") * 3)
+    grad[:300] = 0
+    grad[5000] = float("nan")
+    runs = []
+    for _ in range(2):
+        p = torch.nn.Parameter(torch.zeros(n, device="cuda"))
+        p.grad = grad
+        opt = AdamW([p], betas=(0.5, 0.75), weight_decay=0.0, state_bits=8, rounding="stochastic")
+        opt.step()
+        runs.append({k: v.clone() for k, v in opt.state[p].items()})
+    s = runs[0]
+    for k in s:
+        a, b = (r[k].view(torch.uint8) if r[k].dtype == torch.float8_e4m3fn else r[k] for r in runs)
+        assert torch.equal(a, b), k
+    fine = torch.ones(n, dtype=torch.bool, device="cuda")
+    fine[5000] = False
+    for name, want in (("exp_avg", 0.5 * grad.double()), ("exp_rms", 0.5 * grad.double().abs())):
+        got, per = deq(s, name)
+        q = s[name].double()
+        y = want / per.clamp(min=1e-300)  # exact value in units of the scale
+        place = 2 * half_step(torch.minimum(q.abs(), y.abs()))
+        err = (q - y)[fine]
+        assert (err.abs() <= place[fine] * (1 + 1e-4) + y.abs()[fine] * 1e-6).all()
+        assert (q[:256] == 0).all() and torch.isnan(q[5000])
+        # mean error: below five standard deviations of n draws of at most half a place each way, element by element
+        mid = fine & (y.abs() > 2.0 ** -5)  # the floor of the roots aside
+        z = ((q - y) / place)[mid]
+        assert abs(float(z.mean())) <= 5 * 0.5 / math.sqrt(z.numel())
+        up = float((z > 0).double().mean())
+        assert 0.4 < up < 0.6
+    assert (s["exp_rms"].float()[300:5000] > 0).all()
+    first = s["exp_avg"].view(torch.uint8)
+    opt.step()  # another step, other bits
+    assert float((opt.state[p]["exp_avg"].view(torch.uint8) != first).double().mean()) > 0.2
+
+
+def test_stochastic_rounding_follows_gradients_that_nearest_rounding_loses():
+    """Half of a block's elements stop receiving gradients, the others go on as before: after two thousand steps at beta2 =
+    0.999 the exact root of those is their gradient.  Each stochastic root is a chain of steps of at most 1/8 of it, taken
+    with probabilities below 0.005, whose stationary spread is some 15 %: over 8192 elements the mean is within 10 %, and
+    nine in ten are within 50 %.  Rounded to nearest they sink with the scale of the block."""
+    from fast_jtnn_hip import AdamW
+
+    n = 1 << 14
+    roots = {}
+    for rounding in ("nearest", "stochastic"):
+        p = torch.nn.Parameter(torch.zeros(n, device="cuda"))
+        opt = AdamW([p], lr=0.0, weight_decay=0.0, state_bits=8, rounding=rounding)
+        even = torch.arange(n, device="cuda") % 2 == 0
+        p.grad = torch.where(even, 3.0, 1.0)
+        for _ in range(1000):
+            opt.step()
+        p.grad = torch.where(even, 0.0, 1.0)
+        for _ in range(2000):
+            opt.step()
+        got, _ = deq(opt.state[p], "exp_rms")
+        roots[rounding] = got[~even] / math.sqrt(1 - 0.999 ** 3000)
+    r = roots["stochastic"]
+    assert abs(float(r.mean()) - 1) < 0.1 and float(((r - 1).abs() < 0.5).double().mean()) > 0.9
+    assert float(roots["nearest"].mean()) < 0.6
+
+
 def test_state_dicts():
     """Round trip through a file (both kinds of state), continuing bit for bit; a dict of torch's own optimizer; refusals."""
     from fast_jtnn_hip import AdamW

@@ -87,6 +87,7 @@ def test_adamw_arguments_refused():
     for params, kw, error in (([p(2)], dict(lr=-1.0), ValueError), ([p(2)], dict(betas=(1.0, 0.9)), ValueError),
                               ([p(2)], dict(betas=(0.9, -0.1)), ValueError), ([p(2)], dict(eps=-1e-8), ValueError),
                               ([p(2)], dict(weight_decay=-1), ValueError), ([p(2)], dict(state_bits=16), ValueError),
+                              ([p(2)], dict(rounding="up"), ValueError),
                               ([p(2)], dict(max_norm=0.0), ValueError), ([p(2)], dict(max_norm=float("nan")), ValueError),
                               ([p(2, dtype=torch.float64)], {}, TypeError),
                               ([p(2), p(2, dtype=torch.bfloat16)], {}, TypeError),
@@ -159,7 +160,7 @@ def test_c_entry_points_refuse_before_launch():
 
     def group(**kw):
         a = dict(tensors=256, chunks=256, chunk_ptr=ctypes.addressof(ptr), grads=ctypes.addressof(grads), steps=256,
-                 bias=256, n_tensors=1, n_chunks=1, dtype=K.F32, state_bits=32, use_master=0, lr_device=None, lr=1e-3,
+                 bias=256, n_tensors=1, n_chunks=1, dtype=K.F32, state_bits=32, use_master=0, stochastic=0, lr_device=None, lr=1e-3,
                  beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.0)
         a.update(kw)
         return K.AdamwGroup(*[a[n] for n, _ in K.AdamwGroup._fields_])
