@@ -774,9 +774,12 @@ int jtvae_label_log_probs_bwd(const jtvae_logits_t* logits, const int32_t* owner
   if ((uintptr_t)dx % (logits->dtype == JTVAE_F32 ? 4 : 2)) return JTVAE_E_ALIGN;
   hipStream_t s = (hipStream_t)stream;
   switch (logits->dtype) {
-    case JTVAE_F32: return row_grad<float>(logits, owner, stats, coef, upstream, unless_one, dx, ld_dx, width, scaled, n_scaled, s);
-    case JTVAE_F16: return row_grad<_Float16>(logits, owner, stats, coef, upstream, unless_one, dx, ld_dx, width, scaled, n_scaled, s);
-    default: return row_grad<__bf16>(logits, owner, stats, coef, upstream, unless_one, dx, ld_dx, width, scaled, n_scaled, s);
+    case JTVAE_F32:
+      return row_grad<float>(logits, owner, stats, coef, upstream, unless_one, dx, ld_dx, width, scaled, n_scaled, s);
+    case JTVAE_F16:
+      return row_grad<_Float16>(logits, owner, stats, coef, upstream, unless_one, dx, ld_dx, width, scaled, n_scaled, s);
+    default:
+      return row_grad<__bf16>(logits, owner, stats, coef, upstream, unless_one, dx, ld_dx, width, scaled, n_scaled, s);
   }
 }
 

@@ -37,7 +37,6 @@ struct Words<16> {
 };
 template <>
 struct Words<8> {
-  typedef unsigned at4 __attribute__((ext_vector_type(2), aligned(4)));
   typedef unsigned at2 __attribute__((ext_vector_type(2), aligned(2)));
 };
 template <typename T, int N, bool TWO = sizeof(T) == 2>

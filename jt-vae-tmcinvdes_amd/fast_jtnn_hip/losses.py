@@ -233,7 +233,8 @@ class _Gradient:
 
     def __init__(self, x, labels, g, keep, want, made=False):
         """``made``: the buffer will hold the gradient for an upstream factor of one when the forward pass ends."""
-        self.g, self.keep, self.x_at, self.y_at, self.buffer, self.made = g, keep, x.data_ptr(), labels.data_ptr(), None, made
+        self.g, self.keep, self.x_at, self.y_at = g, keep, x.data_ptr(), labels.data_ptr()
+        self.buffer, self.made = None, made
         if want and (made or g.n_rows * g.n_cols * x.element_size() <= self.EARLY_BYTES):
             self.buffer, self.ld = _grad_rows(x)
 

@@ -10,12 +10,13 @@ per parameter instead of 8.  Such a value has three bits behind the point, and a
 less than half a place: rounded to nearest, an element's share in its block stands still until a gradient is eight to
 eleven times its root, and only the block's scale follows the gradients.  ``rounding="stochastic"`` rounds to one of the
 two neighbours with the right mean instead (by bits that are a function of element, tensor and step: runs repeat), so
-that every element follows its own gradients, within some 15 % of the root.  16-bit parameters are stepped on an fp32 copy (``master=True``), since a step is usually
-smaller than half their last place.
+that every element follows its own gradients, within some 15 % of the root.  16-bit parameters are stepped on an fp32
+copy (``master=True``), since a step is usually smaller than half their last place.
 """
 from __future__ import annotations
 
 import ctypes as C
+import operator
 
 import numpy as np
 import torch
@@ -24,6 +25,7 @@ from . import _capi as K
 from .losses import guard
 
 _E4M3 = torch.float8_e4m3fn
+_GRAD, _DTYPE = operator.attrgetter("grad"), operator.attrgetter("dtype")
 _SCALED = ("exp_avg_scale", "exp_rms_scale")
 
 
@@ -87,7 +89,7 @@ class _Group:
 
     def bind(self):
         """The device table of addresses; rebuilt only when a parameter's storage has moved."""
-        addresses = [p.data_ptr() for p in self.params]
+        addresses = list(map(torch.Tensor.data_ptr, self.params))
         if addresses == self.addresses:
             return
         for p, n in zip(self.params, self.numels):
@@ -107,13 +109,14 @@ class _Group:
 
     def gather_grads(self):
         """Fills the address list; (parameters with a gradient, tensors to keep alive until the launches)."""
-        grads, dt = [p.grad for p in self.params], self.dtype
-        try:  # the usual case in three passes without a branch: every parameter has a plain gradient
-            plain = [g.numel() for g in grads] == self.numels and all([g.dtype is dt and g.is_contiguous() for g in grads])
-        except AttributeError:
+        grads, dt, T = list(map(_GRAD, self.params)), self.dtype, torch.Tensor
+        try:  # the usual case in passes without Python code of their own: every parameter has a plain gradient
+            plain = list(map(T.numel, grads)) == self.numels and all(map(T.is_contiguous, grads)) \
+                and set(map(_DTYPE, grads)) == {dt}
+        except TypeError:  # None among them
             plain = False
         if plain:
-            self.grads[:] = [g.data_ptr() for g in grads]
+            self.grads[:] = list(map(T.data_ptr, grads))
             return self.params, grads
         if any(g is not None and g.numel() != n for g, n in zip(grads, self.numels)):
             raise RuntimeError("AdamW: a gradient has another size than its parameter had when the optimizer was built")
@@ -144,11 +147,11 @@ class AdamW(torch.optim.Optimizer):
         m = beta1 m + (1 - beta1) g,   v = beta2 v + (1 - beta2) g^2,
         w = w (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps).
 
-    ``state_bits``: 32, or 8; ``rounding`` of 8-bit states: "nearest" or "stochastic" (see the module).  ``master``: 16-bit parameters keep an fp32 copy that the step works on; it
-    is the optimizer's, so a value written into such a parameter from outside needs ``refresh_master()``.  ``max_norm``:
-    gradients are multiplied by ``min(1, max_norm / (norm + 1e-6))``, norm being the 2-norm over all parameters of all
-    groups - inside the step, ``.grad`` keeps what backward left; ``grad_norm`` (a 0-d device tensor) holds the norm of
-    the last step.  All parameters are contiguous, on one GPU, of one type per group; a parameter without a gradient is
+    ``state_bits``: 32, or 8; ``rounding`` of 8-bit states: "nearest" or "stochastic" (see the module).  ``master``:
+    16-bit parameters keep an fp32 copy that the step works on; it is the optimizer's, so a value written into such a
+    parameter from outside needs ``refresh_master()``.  ``max_norm``: gradients are multiplied by
+    ``min(1, max_norm / (norm + 1e-6))``, norm being the 2-norm over all parameters of all groups - inside the step,
+    ``.grad`` keeps what backward left; ``grad_norm`` (a 0-d device tensor) holds the norm of the last step.  All parameters are contiguous, on one GPU, of one type per group; a parameter without a gradient is
     left alone.  A captured step replays with the gradients' addresses of the capture; a learning rate that changes
     between replays is a float32 tensor on the device."""
 
