@@ -65,7 +65,8 @@ class _Group:
         chunks = np.stack([of, np.arange(self.n_chunks) - self.chunk_ptr[of]], axis=1).astype(np.int32)
         self.chunks = torch.from_numpy(chunks.reshape(-1) if chunks.size else np.zeros(2, np.int32)).to(dev)
         self.partials = zeros(max(self.n_chunks, 1), torch.float64)
-        self.addresses, self.table, self.versioned = None, None, None
+        self.addresses = None
+        self.table = zeros(C.sizeof(K.AdamwTensor) * len(params), torch.uint8)
         self.grads = (C.c_void_p * len(params))()
         self.views = [self._views(i) for i in range(len(params))]
         if self.master:
@@ -88,7 +89,7 @@ class _Group:
                 self.views[i]["master"].copy_(p.detach())
 
     def bind(self):
-        """The device table of addresses; rebuilt only when a parameter's storage has moved."""
+        """The device table of addresses; written again, in its place, only when a parameter's storage has moved."""
         addresses = list(map(torch.Tensor.data_ptr, self.params))
         if addresses == self.addresses:
             return
@@ -104,7 +105,7 @@ class _Group:
             items[i] = K.AdamwTensor(addresses[i], K.ptr(v.get("master")), v["exp_avg"].data_ptr(), v[second].data_ptr(),
                                      K.ptr(v.get("exp_avg_scale")), K.ptr(v.get("exp_rms_scale")), self.numels[i])
         host = np.frombuffer(bytes(items), dtype=np.uint8).copy()
-        self.table = torch.from_numpy(host).to(self.device)
+        self.table.copy_(torch.from_numpy(host))
         self.addresses = addresses
 
     def gather_grads(self):
@@ -151,9 +152,10 @@ class AdamW(torch.optim.Optimizer):
     16-bit parameters keep an fp32 copy that the step works on; it is the optimizer's, so a value written into such a
     parameter from outside needs ``refresh_master()``.  ``max_norm``: gradients are multiplied by
     ``min(1, max_norm / (norm + 1e-6))``, norm being the 2-norm over all parameters of all groups - inside the step,
-    ``.grad`` keeps what backward left; ``grad_norm`` (a 0-d device tensor) holds the norm of the last step.  All parameters are contiguous, on one GPU, of one type per group; a parameter without a gradient is
-    left alone.  A captured step replays with the gradients' addresses of the capture; a learning rate that changes
-    between replays is a float32 tensor on the device."""
+    ``.grad`` keeps what backward left; ``grad_norm`` (a 0-d device tensor) holds the norm of the last step.  All
+    parameters are contiguous, on one GPU, of one type per group; a parameter without a gradient is left alone.  A
+    captured step replays with the gradients' addresses of the capture; a learning rate that changes between replays is a
+    float32 tensor on the device."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, master=True,
                  max_norm=None, rounding="nearest"):

@@ -480,6 +480,28 @@ def test_captured_and_replayed():
         assert int(first.state[a[0]]["step"]) == 5
 
 
+def test_captured_step_follows_moved_parameters():
+    """The table that a captured step reads is written in its place: after an eager step has seen new storage, replays step
+    that storage."""
+    from fast_jtnn_hip import AdamW
+
+    p = torch.nn.Parameter(torch.ones(5000, device="cuda"))
+    p.grad = torch.ones_like(p)
+    opt = AdamW([p], lr=0.25, weight_decay=0.0)
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    old = p.data
+    p.data = torch.full_like(old, 8.0)
+    opt.step()
+    before = old.clone()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+    assert torch.equal(old, before) and ((p.detach() - 7.0).abs() < 1e-5).all()
+
+
 def test_capture_needs_a_step_first():
     """Refused on the host: nothing has been launched when the error comes."""
     from unittest import mock
