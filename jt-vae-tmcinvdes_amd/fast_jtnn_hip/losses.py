@@ -253,16 +253,23 @@ class _Gradient:
         return d
 
 
+def _tokens(x, labels):
+    """(log-probabilities, buffer of the statistics, jtvae_logits_t, labels it names)."""
+    dev, n = x.device, x.shape[0]
+    lp = torch.empty((n,), dtype=torch.float32, device=dev)
+    buf, (stats,) = _scratch(dev, n)
+    g, keep = _arg(x, labels)
+    K.label_log_probs(g, None, stats, lp.data_ptr(), None)
+    return lp, buf, g, keep
+
+
 class _TokenLogProbs(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, labels, want):
-        x, dev, n = _rows(logits), logits.device, logits.shape[0]
-        with guard(dev):
-            lp = torch.empty((n,), dtype=torch.float32, device=dev)
-            ctx.ws, (stats,) = _scratch(dev, n)
-            g, keep = _arg(x, labels)
-            K.label_log_probs(g, None, stats, lp.data_ptr(), None)
-            ctx.gradient = _Gradient(x, labels, g, keep, want)
+    def forward(ctx, logits, labels):
+        x = _rows(logits)
+        with guard(x.device):
+            lp, ctx.ws, g, keep = _tokens(x, labels)
+            ctx.gradient = _Gradient(x, labels, g, keep, True)
         ctx.save_for_backward(x, labels)
         return lp
 
@@ -271,27 +278,37 @@ class _TokenLogProbs(torch.autograd.Function):
     def backward(ctx, dlp):
         x, labels = ctx.saved_tensors
         coef = dlp.contiguous()
-        return ctx.gradient(x, labels, None, ctx.ws.data_ptr(), coef.data_ptr(), None), None, None
+        return ctx.gradient(x, labels, None, ctx.ws.data_ptr(), coef.data_ptr(), None), None
 
 
 def token_log_probs(logits: torch.Tensor, labels: torch.Tensor) -> torch.Tensor:
     """[N] fp32: log softmax(logits[i])[labels[i]], 0 where the label is negative.  Differentiable in ``logits``."""
     _check("token_log_probs", logits, labels)
     _on_device("token_log_probs", logits, labels=labels)
-    return _TokenLogProbs.apply(logits, labels, _wants_grad(logits))
+    if _wants_grad(logits):
+        return _TokenLogProbs.apply(logits, labels)
+    with guard(logits.device):  # scoring: nothing to record
+        return _tokens(_rows(logits), labels)[0]
+
+
+def _sequences(x, labels, plan):
+    """(sums, buffer that begins with the statistics, jtvae_logits_t, labels it names)."""
+    dev, n = x.device, x.shape[0]
+    plan.on_current_stream()
+    sums = torch.empty((plan.n_seq,), dtype=torch.float32, device=dev)
+    buf, (stats, ws) = _scratch(dev, n, n)
+    g, keep = _arg(x, labels)
+    K.sequence_log_probs(g, plan.arg, stats, sums.data_ptr(), ws, 8 * n)
+    return sums, buf, g, keep
 
 
 class _SequenceLogProbs(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, labels, plan, want):
-        x, dev, n = _rows(logits), logits.device, logits.shape[0]
-        with guard(dev):
-            plan.on_current_stream()
-            sums = torch.empty((plan.n_seq,), dtype=torch.float32, device=dev)
-            ctx.ws, (stats, ws) = _scratch(dev, n, n)
-            g, keep = _arg(x, labels)
-            K.sequence_log_probs(g, plan.arg, stats, sums.data_ptr(), ws, 8 * n)
-            ctx.gradient = _Gradient(x, labels, g, keep, want)
+    def forward(ctx, logits, labels, plan):
+        x = _rows(logits)
+        with guard(x.device):
+            sums, ctx.ws, g, keep = _sequences(x, labels, plan)
+            ctx.gradient = _Gradient(x, labels, g, keep, True)
         ctx.save_for_backward(x, labels)
         ctx.plan = plan
         return sums
@@ -302,7 +319,7 @@ class _SequenceLogProbs(torch.autograd.Function):
         x, labels = ctx.saved_tensors
         stats, coef = ctx.ws.data_ptr(), dsums.contiguous()
         # without sequences no row counts and the coefficients are never read: any address will do
-        return ctx.gradient(x, labels, ctx.plan.arg.row_seq, stats, coef.data_ptr() or stats, None), None, None, None
+        return ctx.gradient(x, labels, ctx.plan.arg.row_seq, stats, coef.data_ptr() or stats, None), None, None
 
 
 def sequence_log_probs(logits: torch.Tensor, labels: torch.Tensor, plan: SequencePlan) -> torch.Tensor:
@@ -311,7 +328,10 @@ def sequence_log_probs(logits: torch.Tensor, labels: torch.Tensor, plan: Sequenc
     _check("sequence_log_probs", logits, labels)
     _check_plan("sequence_log_probs", plan, logits)
     _on_device("sequence_log_probs", logits, labels=labels, plan=plan)
-    return _SequenceLogProbs.apply(logits, labels, plan, _wants_grad(logits))
+    if _wants_grad(logits):
+        return _SequenceLogProbs.apply(logits, labels, plan)
+    with guard(logits.device):  # scoring: nothing to record
+        return _sequences(_rows(logits), labels, plan)[0]
 
 
 class _PreferenceLoss(torch.autograd.Function):
