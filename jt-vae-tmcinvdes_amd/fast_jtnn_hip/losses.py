@@ -225,25 +225,30 @@ class _Gradient:
     """The gradient of a call's logits.  What can be made ready is made with the forward pass: autograd runs the backward
     pass on a thread of its own, which has just been woken and takes two to three times as long over the same Python.
     Buffers of up to ``EARLY_BYTES`` are among it (24 x 385, both passes: 112 -> 90 us on one machine); larger ones
-    are not held between the passes."""
+    are not held between the passes.  Nothing made early serves where one of the passes is captured into a graph and the
+    other is not: a replay would write a buffer that is no memory of the graph's, or find one that has been changed."""
 
     EARLY_BYTES = 4 << 20
 
-    __slots__ = ("g", "keep", "x_at", "y_at", "buffer", "ld", "made")
+    __slots__ = ("g", "keep", "x_at", "y_at", "buffer", "ld", "made", "captured")
 
     def __init__(self, x, labels, g, keep, want, made=False):
         """``made``: the buffer will hold the gradient for an upstream factor of one when the forward pass ends."""
         self.g, self.keep, self.x_at, self.y_at = g, keep, x.data_ptr(), labels.data_ptr()
-        self.buffer, self.made = None, made
+        self.buffer, self.made, self.captured = None, made, torch.cuda.is_current_stream_capturing()
         if want and (made or g.n_rows * g.n_cols * x.element_size() <= self.EARLY_BYTES):
             self.buffer, self.ld = _grad_rows(x)
+
+    def early(self, buffer):
+        """A buffer made with the forward pass, if the backward pass that now runs may use it."""
+        return buffer if buffer is not None and self.captured == torch.cuda.is_current_stream_capturing() else None
 
     def __call__(self, x, labels, owner, stats, coef, up, scaled=None, n_scaled=0):
         """The gradient from saved statistics and coefficients (addresses), on the device and stream of the forward pass,
         which autograd has made the current ones."""
-        d, self.buffer = self.buffer, None
+        d, self.buffer = self.early(self.buffer), None
         unless_one = self.made and d is not None
-        if d is None:  # not held, or given away by an earlier pass through the same graph
+        if d is None:  # not held or not fit, or given away by an earlier pass through the same graph
             d, self.ld = _grad_rows(x)
         if x.data_ptr() != self.x_at or labels.data_ptr() != self.y_at:  # saved tensors may come back at another place
             self.g, self.keep = _arg(x, labels)
@@ -364,7 +369,7 @@ class _PreferenceLoss(torch.autograd.Function):
         x, labels = ctx.saved_tensors
         plan, d, (stats, coef) = ctx.plan, None, ctx.at
         want, want_other = ctx.needs_input_grad[:2]
-        dother, ctx.dother = ctx.dother, None
+        dother, ctx.dother = ctx.gradient.early(ctx.dother), None
         if want_other and dother is None:  # a second pass through the graph
             dother = torch.empty((plan.n_seq,), dtype=torch.float32, device=x.device)
         if want:

@@ -553,6 +553,40 @@ def test_captured_and_replayed(n, v, dtype):
             assert torch.equal(a, b), (k, i)
 
 
+def test_backward_captured_alone():
+    """An eager forward pass whose backward pass is captured: every replay writes the whole gradient, into memory of the
+    graph's own, whatever became of the last replay's."""
+    from fast_jtnn_hip import SequencePlan, policy_loss, preference_loss, sequence_log_probs, token_log_probs
+
+    n, v = 24, 385
+    x, labels = make(n, v, torch.float32, 15)
+    x = x.contiguous().requires_grad_()
+    plan = SequencePlan(np.arange(n) % 4, 4, "cuda", pairs=[[0, 1], [2, 3]])
+    ref, adv = torch.zeros(4, device="cuda"), torch.randn(n, device="cuda")
+    old = torch.full((n,), -3.0, device="cuda")
+    other = torch.zeros(4, device="cuda", requires_grad=True)
+    calls = [(lambda: token_log_probs(x, labels).sum(), [x]),
+             (lambda: sequence_log_probs(x, labels, plan).sum(), [x]),
+             (lambda: preference_loss(x, labels, plan, ref, other_log_probs=other).loss, [x, other]),
+             (lambda: policy_loss(x, labels, old, adv).loss, [x])]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        losses = [f() for f, _ in calls]
+        want = [torch.autograd.grad(f(), leaves) for f, leaves in calls]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        got = [torch.autograd.grad(loss, leaves, retain_graph=True) for loss, (_, leaves) in zip(losses, calls)]
+    for k in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        for i, (a, b) in enumerate(zip(got, want)):
+            for p, q in zip(a, b):
+                assert torch.equal(p, q), (k, i)
+                p.fill_(float("nan"))
+
+
 def test_more_rows_than_one_launch_takes():
     """68 million rows of two columns: more work-items than a grid may have, so several launches."""
     from fast_jtnn_hip import policy_loss, token_log_probs
