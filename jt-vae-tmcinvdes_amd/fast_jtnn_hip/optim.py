@@ -15,6 +15,7 @@ copy (``master=True``), since a step is usually smaller than half their last pla
 """
 from __future__ import annotations
 
+import copy
 import ctypes as C
 import operator
 
@@ -97,6 +98,9 @@ class _Group:
             if p.device != self.device or p.dtype != self.dtype or p.numel() != n or not p.is_contiguous():
                 raise RuntimeError("AdamW: a parameter changed its device, type, size or layout after the optimizer "
                                    "was built; build it again")
+        spans = sorted((a, a + n * p.element_size()) for a, n, p in zip(addresses, self.numels, self.params) if n)
+        if any(end > start for (_, end), (start, _) in zip(spans, spans[1:])):
+            raise RuntimeError("AdamW: parameters of one group share memory; a step would work on it twice at once")
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW: the parameters' addresses must be known before a capture; make one step first")
         items = (K.AdamwTensor * len(self.params))()
@@ -153,9 +157,9 @@ class AdamW(torch.optim.Optimizer):
     parameter from outside needs ``refresh_master()``.  ``max_norm``: gradients are multiplied by
     ``min(1, max_norm / (norm + 1e-6))``, norm being the 2-norm over all parameters of all groups - inside the step,
     ``.grad`` keeps what backward left; ``grad_norm`` (a 0-d device tensor) holds the norm of the last step.  All
-    parameters are contiguous, on one GPU, of one type per group; a parameter without a gradient is left alone.  A
-    captured step replays with the gradients' addresses of the capture; a learning rate that changes between replays is a
-    float32 tensor on the device."""
+    parameters are contiguous and on one GPU, those of a group of one type and without memory in common; a parameter
+    without a gradient is left alone.  A captured step replays with the gradients' addresses of the capture; a learning
+    rate that changes between replays is a float32 tensor on the device."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, master=True,
                  max_norm=None, rounding="nearest"):
@@ -190,6 +194,8 @@ class AdamW(torch.optim.Optimizer):
             self._check_hyper(g)
             if g["state_bits"] not in (8, 32):
                 raise ValueError("AdamW: state_bits is 32 or 8, got %r" % (g["state_bits"],))
+            if len(set(g["params"])) != len(g["params"]):
+                raise ValueError("AdamW: a parameter appears twice in a group")
             for p in g["params"]:
                 if p.dtype not in K.DTYPE_CODE:
                     raise TypeError("AdamW: parameters are float32, float16 or bfloat16, got %s" % p.dtype)
@@ -214,6 +220,9 @@ class AdamW(torch.optim.Optimizer):
         self._bound.append(group)
         for p, v in zip(group.params, group.views):
             self.state[p] = v
+
+    def __getstate__(self):
+        raise TypeError("AdamW cannot be copied or pickled (its tables hold addresses): use state_dict()")
 
     @property
     def grad_norm(self):
@@ -266,8 +275,9 @@ class AdamW(torch.optim.Optimizer):
     @torch.no_grad()
     def load_state_dict(self, state_dict):
         """Takes the states of a dict of the same parameter groups (this class's, or with ``state_bits=32`` that of
-        ``torch.optim.AdamW`` / ``Adam``) into the buffers; hyperparameters follow the dict, ``state_bits`` and ``master``
-        do not.  A parameter without an entry starts afresh."""
+        ``torch.optim.AdamW`` / ``Adam`` without the variants that this class does not step by) into the buffers;
+        hyperparameters follow the dict, ``state_bits`` and ``master`` do not.  A learning rate on the device takes its
+        new value in its place.  A parameter without an entry starts afresh."""
         groups = state_dict["param_groups"]
         if len(groups) != len(self.param_groups):
             raise ValueError("AdamW: the state dict has %d parameter groups, the optimizer %d"
@@ -276,6 +286,11 @@ class AdamW(torch.optim.Optimizer):
             if len(new["params"]) != len(g.params):
                 raise ValueError("AdamW: a group of the state dict has %d parameters, the optimizer's %d"
                                  % (len(new["params"]), len(g.params)))
+            for k in ("amsgrad", "maximize"):
+                if new.get(k):
+                    raise ValueError("AdamW: the state dict's %s is not offered" % k)
+            if new.get("weight_decay") and not new.get("decoupled_weight_decay", True):
+                raise ValueError("AdamW: the state dict's weight decay is part of its gradients, not decoupled")
         todo = []
         for new, g in zip(groups, self._bound):
             for i, key in enumerate(new["params"]):
@@ -307,4 +322,7 @@ class AdamW(torch.optim.Optimizer):
                 else:
                     dst.zero_()
         for new, mine in zip(groups, self.param_groups):
-            mine.update({k: v for k, v in new.items() if k not in ("params", "state_bits", "master")})
+            lr = mine["lr"]
+            mine.update({k: copy.deepcopy(v) for k, v in new.items() if k not in ("params", "state_bits", "master")})
+            if isinstance(lr, torch.Tensor):  # a captured step reads it where it is
+                mine["lr"] = lr.fill_(float(mine["lr"]))

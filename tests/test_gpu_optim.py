@@ -354,6 +354,50 @@ def test_state_dicts():
         assert torch.equal(opt.state[p]["exp_avg"], m)  # a refused dict changes nothing
 
 
+def test_state_dicts_of_other_rules_refused():
+    """Another optimizer's variants; a learning rate on the device takes a dict's value where it is."""
+    from fast_jtnn_hip import AdamW
+
+    for rule, kw, ok in ((torch.optim.AdamW, dict(amsgrad=True), False), (torch.optim.AdamW, dict(maximize=True), False),
+                         (torch.optim.Adam, dict(weight_decay=0.1), False), (torch.optim.Adam, {}, True),
+                         (torch.optim.AdamW, dict(weight_decay=0.1), True)):
+        ps = params_of(SHAPES[1:4], torch.float32, 7)
+        ref = rule(ps, lr=0.5, **kw)
+        ref.step()
+        lr = torch.tensor(0.25, device="cuda")
+        opt = AdamW(ps, lr=lr)
+        if ok:
+            opt.load_state_dict(ref.state_dict())
+            assert opt.param_groups[0]["lr"] is lr and float(lr) == 0.5
+            assert opt.param_groups[0]["weight_decay"] == kw.get("weight_decay", 0)
+        else:
+            with pytest.raises(ValueError):
+                opt.load_state_dict(ref.state_dict())
+            assert float(lr) == 0.25 and int(opt.state[ps[0]]["step"]) == 0
+    other = AdamW(ps, lr=torch.tensor(1.0, device="cuda"))
+    other.load_state_dict(opt.state_dict())
+    lr.fill_(3.0)
+    assert float(other.param_groups[0]["lr"]) == 0.5
+    with pytest.raises(TypeError, match="state_dict"):
+        copy.deepcopy(opt)
+
+
+def test_parameters_that_share_memory_refused():
+    from fast_jtnn_hip import AdamW
+
+    buf = torch.ones(512, device="cuda")
+    for a, b, ok in ((buf[:256], buf[256:], True), (buf[:256], buf[255:], False), (buf, buf, False),
+                     (buf[100:101], buf[:512], False), (buf[300:300], buf, True)):
+        a, b = torch.nn.Parameter(a), torch.nn.Parameter(b)
+        a.grad, b.grad = torch.ones_like(a), torch.ones_like(b)
+        opt = AdamW([a, b])
+        if ok:
+            opt.step()
+        else:
+            with pytest.raises(RuntimeError, match="share memory"):
+                opt.step()
+
+
 def test_works_with_schedulers_strided_gradients_and_closures():
     from fast_jtnn_hip import AdamW
 

@@ -96,6 +96,14 @@ def test_adamw_arguments_refused():
             AdamW(params, **kw)
 
 
+@pytest.mark.filterwarnings("ignore:optimizer contains")
+def test_adamw_refuses_a_parameter_given_twice():
+    """Two blocks would work on its elements at once."""
+    p = torch.nn.Parameter(torch.zeros(2))
+    with pytest.raises(ValueError, match="twice"):
+        AdamW([p, torch.nn.Parameter(torch.zeros(2)), p])
+
+
 def test_c_entry_points_refuse_before_launch():
     lib = K.lib
     ok = K.Logits(256, K.F32, 8, 4, 7, 256, 64)
