@@ -534,7 +534,7 @@ int jtvae_label_log_probs(const jtvae_logits_t* logits, const int32_t* owner, fl
                           double* log_probs64, void* stream);
 
 /* dx[i, j] = c_i ([j = label_i] - softmax(x_i)_j) in the logits' type, c_i = coef[owner ? owner[i] : i] * upstream
- * (device scalar, or NULL = 1); rows without a label get zeros.  Columns [n_cols, width) are padding and
+ * (device scalar, or NULL = 1); rows without a label or with c_i = 0 get zeros, whatever they hold.  Columns [n_cols, width) are padding and
  * become zero (n_cols <= width <= ld_dx).  unless_one: dx holds the gradient for upstream = 1 already and stays
  * as it is if *upstream is 1.  scaled (n_scaled > 0): scaled[q] = coef[q] * upstream. */
 int jtvae_label_log_probs_bwd(const jtvae_logits_t* logits, const int32_t* owner, const float* stats,
@@ -584,6 +584,7 @@ typedef struct jtvae_policy {
 /* r = exp(lp - old), k3 = exp(ref - lp) - (ref - lp) - 1, w = scale * weights:
  * *loss = sum w (kl_coef k3 - min(r A, clip(r) A)) over the rows with a label, *kl = sum w k3, *clipped = sum of w over
  * the rows whose ratio was clipped (device scalars); coef[i] = d loss / d lp_i; log_probs and stats as above.
+ * A row of weight zero has no part in any of them but log_probs and stats, whatever it and its inputs hold.
  * dx (or NULL): the gradient of loss with respect to the logits, as jtvae_label_log_probs_bwd gives it. */
 size_t jtvae_policy_loss_workspace_bytes(int32_t n_rows);
 int jtvae_policy_loss(const jtvae_logits_t* logits, const jtvae_policy_t* policy, float* stats, float* log_probs,

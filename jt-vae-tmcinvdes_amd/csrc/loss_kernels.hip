@@ -5,7 +5,9 @@
 // d(log p_l)/dx_j = [j = l] - exp(x_j - m) / s.  Statistics are fp32; the one value per row that is compared with
 // other models' values (log p_l) is formed in fp64, because sequences sum thousands of them and take differences.
 // A row without a label (label < 0, or owner < 0 where owners are given) is not read: log-probability 0, gradient 0.
-// A label >= V gives NaN (the call cannot look at device memory without a wait).
+// A label >= V gives NaN (the call cannot look at device memory without a wait).  A coefficient of zero gives a gradient
+// of zero, and a weight of zero no term of a loss, whatever else the row holds: masks come that way, and behind them may
+// be infinities and NaN.
 #include "../../include/jtvae_hip.h"
 #include "jtvae_common.h"
 
@@ -153,8 +155,9 @@ struct PolicyIn {
 };
 
 __device__ __forceinline__ PolicyRow policy_row(const PolicyIn& in, int row, double lp) {
-  PolicyRow o;
+  PolicyRow o = {0.0, 0.0, 0.0, 0.f};
   const double w = in.scale * (in.weights ? (double)in.weights[row] : 1.0);
+  if (w == 0.0) return o;
   const double a = (double)in.adv[row], r = exp(lp - (double)in.old_lp[row]);
   const double plain = r * a, cut = (r < in.lo ? in.lo : (r > in.hi ? in.hi : r)) * a;
   const bool clipped = cut < plain;
@@ -164,10 +167,11 @@ __device__ __forceinline__ PolicyRow policy_row(const PolicyIn& in, int row, dou
     k3 = e - gap;
     dk3 = -e;
   }
-  o.loss = w * (in.kl_coef * k3 - (clipped ? cut : plain));
+  const bool penalty = in.kl_coef > 0.0;  // without one an infinite k3 is reported, not multiplied
+  o.loss = w * ((penalty ? in.kl_coef * k3 : 0.0) - (clipped ? cut : plain));
   o.kl = w * k3;
   o.clipped = clipped ? w : 0.0;
-  o.coef = (float)(w * (in.kl_coef * dk3 - (clipped ? 0.0 : plain)));
+  o.coef = (float)(w * ((penalty ? in.kl_coef * dk3 : 0.0) - (clipped ? 0.0 : plain)));
   return o;
 }
 
@@ -339,7 +343,7 @@ __global__ __launch_bounds__(RT* R, NV > 8 ? 4 : RT == 64 && NV == 8 ? 6 : 8) vo
         terms[mine] = p.loss;
         terms[n_terms + mine] = p.kl;
         terms[2 * n_terms + mine] = p.clipped;
-        end[i] = make_float4(s.m, s.s, l < in.n_cols ? p.coef : NAN, 0.f);
+        end[i] = make_float4(s.m, s.s, p.coef, 0.f);
       }
     }
   }
@@ -350,12 +354,13 @@ __global__ __launch_bounds__(RT* R, NV > 8 ? 4 : RT == 64 && NV == 8 ? 6 : 8) vo
     T* d = out.dx + (long)row * out.ld;
     const float4 f = end[r];
     const float m = finite_or_zero(f.x), k = f.z, ks = k / f.y;
+    const bool due = counted && k != 0.f;
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
       const int i = t + u * RT;
       if (i >= n_vec) break;
       float v[E];
-      if (counted) {
+      if (due) {
         Vec<T>::unpack(w[u], v);
         softmax_grad<E>(v, shape.col(i), label, m, ks, k);
       } else {
@@ -366,7 +371,7 @@ __global__ __launch_bounds__(RT* R, NV > 8 ? 4 : RT == 64 && NV == 8 ? 6 : 8) vo
     }
     if (c_one < (unsigned)in.n_cols) {
       float v = 0.f;
-      if (counted) {
+      if (due) {
         v = one;
         softmax_grad<1>(&v, c_one, label, m, ks, k);
       }
@@ -407,7 +412,7 @@ __global__ __launch_bounds__(JTVAE_BLOCK) void grad_kernel(RowsIn<T> in, const f
     T* d = out.dx + (long)row * out.ld;
     const Shape<T> shape(x, in.n_cols);
     const int n_vec = shape.n_vec, first = tile * RT * NV + t;
-    float k = 0.f, ks = 0.f, m = 0.f;
+    float k = 0.f, ks = 0.f, m = 0.f;  // loads of the row are under way before its coefficient is known
     Word4 w[NV];
     if (counted) {
 #pragma unroll
@@ -415,16 +420,18 @@ __global__ __launch_bounds__(JTVAE_BLOCK) void grad_kernel(RowsIn<T> in, const f
         if (first + u * RT < n_vec)
           w[u] = ONCE ? Vec<T>::load_once(x + shape.col(first + u * RT)) : Vec<T>::load(x + shape.col(first + u * RT));
       const float2 st = in.stats[row];
-      k = label < in.n_cols ? coef[own] * up : NAN;
+      k = coef[own] * up;
+      if (label >= in.n_cols && k != 0.f) k = NAN;
       m = finite_or_zero(st.x);
       ks = k / st.y;
     }
+    const bool due = counted && k != 0.f;
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
       const int i = first + u * RT;
       if (i >= n_vec) break;
       float v[E];
-      if (counted) {
+      if (due) {
         Vec<T>::unpack(w[u], v);
         softmax_grad<E>(v, shape.col(i), label, m, ks, k);
       } else {
@@ -437,7 +444,7 @@ __global__ __launch_bounds__(JTVAE_BLOCK) void grad_kernel(RowsIn<T> in, const f
       const unsigned c = shape.extra(t);
       if (c < (unsigned)in.n_cols) {
         float v = 0.f;
-        if (counted) {
+        if (due) {
           v = (float)x[c];
           softmax_grad<1>(&v, c, label, m, ks, k);
         }

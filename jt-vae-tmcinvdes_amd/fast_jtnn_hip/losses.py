@@ -10,8 +10,9 @@ preferred, learning from rewards of sampled ones - needs the log-probability of 
 * ``policy_loss(...)``: clipped probability ratios with a KL term.
 
 Logits are [N, V] in fp32, fp16 or bf16, rows at any stride; labels are [N] int32 or int64, a negative label leaves its
-row out (log-probability 0, gradient 0, its logits are never read).  A label >= V gives NaN.  Gradients come back in the
-logits' type and layout, and are differentiable once.  Statistics are fp32, sums over a sequence fp64; no atomics, so
+row out (log-probability 0, gradient 0, its logits are never read).  A label >= V gives NaN.  Where the upstream gradient
+or a weight is zero the gradient is zero, whatever the row holds.  Gradients come back in the logits' type and layout, and
+are differentiable once.  Statistics are fp32, sums over a sequence fp64; no atomics, so
 results repeat bit for bit.  Every call only enqueues work on the current stream and may be captured; a captured plan
 lives as long as the graph.
 """
@@ -451,7 +452,8 @@ def policy_loss(logits: torch.Tensor, labels: torch.Tensor, old_log_probs: torch
         loss = scale * sum over rows of weights (kl_coef k - min(r A, min(max(r, 1 - clip), 1 + clip) A)).
 
     ``clip`` is one number or (low, high); without ``ref_log_probs`` there is no KL term (``kl_coef`` must be 0).  Rows
-    with a negative label do not count; ``weights`` (default 1) carry masks and means.  Differentiable in ``logits``; the
+    with a negative label or a weight of zero do not count, whatever their other inputs hold; ``weights`` (default 1) carry
+    masks and means.  Differentiable in ``logits``; the
     other inputs are constants.  The gradient is made along with the loss, for a factor of one on it: a factor is best
     given as ``scale`` (another one in the backward pass is right too, and makes the gradient a second time)."""
     what = "policy_loss"

@@ -382,6 +382,68 @@ def test_policy_loss(n, v, dtype):
         assert (d[labels < 0] == 0).all()
 
 
+@pytest.mark.parametrize("n,v,dtype", [(40, 385, torch.float32), (9, 4099, torch.bfloat16), (6, 30011, torch.float16),
+                                       (4, 70001, torch.float32)])
+def test_nothing_comes_from_behind_a_mask(n, v, dtype):
+    """Weights of zero, upstream gradients of zero and sequences in no pair, over infinities and NaN: the others' values are
+    those of the batch without the masked rows."""
+    from fast_jtnn_hip import SequencePlan, policy_loss, preference_loss, sequence_log_probs, token_log_probs
+
+    x, labels = make(n, v, dtype, n * v)
+    x = x.contiguous()
+    old, adv, ref = torch.full((n,), -3.0, device="cuda"), torch.randn(n, device="cuda"), torch.full((n,), -2.5, device="cuda")
+    masked = torch.arange(n, device="cuda") % 2 == 1
+    w = torch.where(masked, 0.0, 0.5)
+    bad = x.clone()
+    bad[1::2] = float("nan")
+    bad[1] = float("-inf")
+    bad[3, 0] = float("inf")
+    labels[3] = v + 5
+    olds, advs, refs = (torch.where(masked, b, t) for t, b in ((old, -math.inf), (adv, math.nan), (ref, math.inf)))
+    bad.requires_grad_()
+    kept = x[::2].detach().requires_grad_()  # a view: rows at the same distance from 16-byte boundaries, so the same bits
+
+    def same(d, want):
+        assert (d[1::2] == 0).all() and torch.equal(d[::2], want)
+
+    out = policy_loss(bad, labels, olds, advs, ref_log_probs=refs, weights=w, kl_coef=0.1)
+    few = policy_loss(kept, labels[::2], old[::2], adv[::2], ref_log_probs=ref[::2], weights=w[::2], kl_coef=0.1)
+    for f in ("loss", "kl", "clipped"):
+        a, b = float(getattr(out, f)), float(getattr(few, f))
+        assert abs(a - b) <= 2.0 ** -22 * abs(b) and math.isfinite(b)  # the same terms, perhaps in another order
+    for up in (1.0, -2.0):  # made with the forward pass, and made again
+        one = torch.tensor(up, device="cuda")
+        same(torch.autograd.grad(out.loss, bad, one, retain_graph=True)[0],
+             torch.autograd.grad(few.loss, kept, one, retain_graph=True)[0])
+    lp = token_log_probs(bad, labels)
+    a = torch.where(masked, 0.0, lp).sum()
+    same(torch.autograd.grad(a, bad)[0], torch.autograd.grad(token_log_probs(kept, labels[::2]).sum(), kept)[0])
+    a = sequence_log_probs(bad, labels, SequencePlan(np.arange(n) % 2, 2, "cuda"))[0]
+    b = sequence_log_probs(kept, labels[::2], SequencePlan(np.zeros(len(kept), np.int32), 1, "cuda"))[0]
+    assert torch.equal(a, b)
+    same(torch.autograd.grad(a, bad)[0], torch.autograd.grad(b, kept)[0])
+    # sequences 0 and 2 are a pair, 1 and 3 (the masked rows) are in none
+    plan = SequencePlan(np.arange(n) % 4, 4, "cuda", pairs=[[0, 2]])
+    less = SequencePlan(np.arange(n)[::2] % 4 // 2, 2, "cuda", pairs=[[0, 1]])
+    r = preference_loss(bad, labels, plan, torch.tensor([0.0, math.nan, 0.0, math.inf], device="cuda"))
+    q = preference_loss(kept, labels[::2], less, torch.zeros(2, device="cuda"))
+    assert torch.equal(r.loss, q.loss)
+    same(torch.autograd.grad(r.loss, bad)[0], torch.autograd.grad(q.loss, kept)[0])
+
+
+def test_an_infinite_estimate_without_a_penalty():
+    """kl_coef = 0: an infinite KL estimate is reported and does not touch the loss."""
+    from fast_jtnn_hip import policy_loss
+
+    x, labels = make(8, 385, torch.float32, 3)
+    x.requires_grad_()
+    old, adv = torch.full((8,), -2.0, device="cuda"), torch.ones(8, device="cuda")
+    ref = torch.full((8,), -math.inf, device="cuda")
+    out, want = policy_loss(x, labels, old, adv, ref_log_probs=ref), policy_loss(x, labels, old, adv)
+    assert float(out.kl) == math.inf and torch.equal(out.loss, want.loss)
+    assert torch.equal(torch.autograd.grad(out.loss, x)[0], torch.autograd.grad(want.loss, x)[0])
+
+
 def test_no_rows():
     from fast_jtnn_hip import SequencePlan, policy_loss, preference_loss, sequence_log_probs
 
