@@ -214,7 +214,7 @@ __device__ __forceinline__ float round_by(float x, unsigned bits20) {
 // e4m3 values of v over the block's scale.  `dice`: 0 = to nearest, else 20 random bits per element (low 20 bits of each).
 template <bool ROOT>
 __device__ __forceinline__ unsigned quantise(const float v[4], float top, bool by_dice, const unsigned dice[4]) {
-  const float inv = top > kSmallest ? kTop / top : 0.f;
+  const float inv = top > kSmallest ? 1.f / top * kTop : 0.f;
   float x[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
@@ -264,8 +264,9 @@ __device__ __forceinline__ void update(const jtvae_adamw_tensor_t& t, const T* g
   }
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
+    // the order of the elementary operations (decay, then add), which settles where an 8-bit state near a tie goes
     const float x = g[k] * s.grad_scale;
-    m[k] = s.beta1 * m[k] + s.one_m_beta1 * x;
+    m[k] = fmaf(s.one_m_beta1, x, s.beta1 * m[k]);
     v[k] = s.beta2 * v[k] + s.one_m_beta2 * (x * x);
     r[k] = root(v[k]);
     // reciprocal on the hardware unit (1 ulp): the update is off by 2^-22 of itself, below half an ulp of w
