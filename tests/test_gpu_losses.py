@@ -382,6 +382,42 @@ def test_policy_loss(n, v, dtype):
         assert (d[labels < 0] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,v", [(1, 4096), (1, 8191), (1, 8192), (2, 8209), (4, 128000), (64, 20011), (65, 20011), (3, 600011)])
+def test_sums_of_a_few_long_rows(n, v, dtype):
+    """Long rows with others that do not count, -inf, NaN and a single finite logit among them; a row's value is the same
+    among few and alone, and the gradient works from the statistics left behind."""
+    from fast_jtnn_hip import SequencePlan, sequence_log_probs
+
+    x, labels = make(n, v, dtype, n + v, ld=v + 1, offset=1)
+    owner = np.arange(n) % 3
+    x[0, v // 2:] = float("-inf")
+    labels[0] = v // 3
+    if n > 3:
+        owner[1] = -1
+        x[1] = float("nan")
+        x[2] = float("-inf")
+        x[2, v - 1] = 3.0
+        labels[2] = v - 1
+        labels[3] = -1
+    x.requires_grad_()
+    sums = sequence_log_probs(x, labels, SequencePlan(owner, 4, "cuda"))
+    counted = torch.tensor(owner, device="cuda") >= 0
+    keep = torch.where(counted, labels, -1)
+    lp, soft, dist = exact(torch.nan_to_num(x.detach(), nan=0.0, posinf=None, neginf=float("-inf")), keep)
+    want = torch.zeros(4, dtype=torch.float64, device="cuda").index_add_(0, torch.tensor(owner, device="cuda").clamp(min=0), lp)
+    rows = -(-n // 3)
+    assert ((sums.double() - want).abs() <= rows * sum_error(v) + want.abs() * 2.0 ** -23).all()
+    alone = [sequence_log_probs(x[i:i + 1], labels[i:i + 1], SequencePlan([0], 1, "cuda")) for i in range(min(n, 3))]
+    if n <= 3:
+        assert torch.equal(torch.cat(alone), sums[:n])
+    (d,) = torch.autograd.grad(sums.sum(), x)
+    check_grad(d, soft, dist, keep, torch.ones(n, device="cuda"), dtype)
+    bad = x.detach().clone()
+    bad[0, 5] = float("nan")
+    assert torch.isnan(sequence_log_probs(bad[:1], labels[:1], SequencePlan([0], 1, "cuda"))).all()
+
+
 @pytest.mark.parametrize("n,v,dtype", [(40, 385, torch.float32), (9, 4099, torch.bfloat16), (6, 30011, torch.float16),
                                        (4, 70001, torch.float32)])
 def test_nothing_comes_from_behind_a_mask(n, v, dtype):
