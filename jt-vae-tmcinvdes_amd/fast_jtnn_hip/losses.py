@@ -231,14 +231,31 @@ class _Gradient:
 
     EARLY_BYTES = 4 << 20
 
-    __slots__ = ("g", "keep", "x_at", "y_at", "buffer", "ld", "made", "captured")
+    __slots__ = ("g", "keep", "place", "buffer", "ld", "made", "captured")
 
     def __init__(self, x, labels, g, keep, want, made=False):
         """``made``: the buffer will hold the gradient for an upstream factor of one when the forward pass ends."""
-        self.g, self.keep, self.x_at, self.y_at = g, keep, x.data_ptr(), labels.data_ptr()
+        self.g, self.keep, self.place = g, keep, self._place(x, labels)
         self.buffer, self.made, self.captured = None, made, torch.cuda.is_current_stream_capturing()
         if want and (made or g.n_rows * g.n_cols * x.element_size() <= self.EARLY_BYTES):
             self.buffer, self.ld = _grad_rows(x)
+
+    @staticmethod
+    def _place(x, labels):
+        """What ``g`` says of the saved tensors.  The strides belong to it: a copy may take the freed logits' address and
+        lie there without their padding."""
+        return x.data_ptr(), x.stride(), labels.data_ptr()
+
+    def _moved(self, x, labels):
+        """(logits as rows, jtvae_logits_t, labels it names) of saved tensors that come back elsewhere; hooks may return
+        them in any layout, but not as anything else."""
+        what = "backward pass"
+        _check(what, x, labels)
+        _on_device(what, x, labels=labels)
+        if x.shape != (self.g.n_rows, self.g.n_cols) or K.DTYPE_CODE[x.dtype] != self.g.dtype:
+            raise RuntimeError("%s: the saved logits came back as %s %s" % (what, x.dtype, tuple(x.shape)))
+        x = _rows(x)
+        return (x, *_arg(x, labels))
 
     def early(self, buffer):
         """A buffer made with the forward pass, if the backward pass that now runs may use it."""
@@ -251,10 +268,10 @@ class _Gradient:
         unless_one = self.made and d is not None
         if d is None:  # not held or not fit, or given away by an earlier pass through the same graph
             d, self.ld = _grad_rows(x)
-        if x.data_ptr() != self.x_at or labels.data_ptr() != self.y_at:  # saved tensors may come back at another place
-            self.g, self.keep = _arg(x, labels)
-            self.x_at, self.y_at = x.data_ptr(), labels.data_ptr()
-        K.label_log_probs_bwd(self.g, owner, stats, coef, up, d.data_ptr(), self.ld, self.ld, int(unless_one), scaled,
+        g = self.g
+        if self._place(x, labels) != self.place:
+            x, g, labels = self._moved(x, labels)
+        K.label_log_probs_bwd(g, owner, stats, coef, up, d.data_ptr(), self.ld, self.ld, int(unless_one), scaled,
                               n_scaled)
         return d
 
