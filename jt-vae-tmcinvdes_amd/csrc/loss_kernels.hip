@@ -377,7 +377,7 @@ __global__ __launch_bounds__(RT* R, NV > 8 ? 4 : RT == 64 && NV == 8 ? 6 : 8) vo
       }
       d[c_one] = (T)v;
     }
-    for (long c = in.n_cols + t; c < out.width; c += RT) d[c] = (T)0.f;
+    for (long c = (long)in.n_cols + t; c < out.width; c += RT) d[c] = (T)0.f;
   }
 }
 
@@ -450,7 +450,7 @@ __global__ __launch_bounds__(JTVAE_BLOCK) void grad_kernel(RowsIn<T> in, const f
         }
         d[c] = (T)v;
       }
-      for (long p = in.n_cols + t; p < out.width; p += RT) d[p] = (T)0.f;
+      for (long p = (long)in.n_cols + t; p < out.width; p += RT) d[p] = (T)0.f;
     }
   }
 }
@@ -467,7 +467,7 @@ struct Sequences {
 __device__ __forceinline__ double sequence_sum(const Sequences& q, const double* lp64, const float* other, int seq,
                                                int lane) {
   double acc = 0.0;
-  for (int i = q.rowptr[seq] + lane; i < q.rowptr[seq + 1]; i += 64) acc += lp64[q.rows[i]];
+  for (long i = (long)q.rowptr[seq] + lane; i < q.rowptr[seq + 1]; i += 64) acc += lp64[q.rows[i]];
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) acc += __shfl_xor(acc, off, 64);
   return other ? acc + (double)other[seq] : acc;

@@ -34,3 +34,26 @@ def test_saved_logits_without_their_padding():
             loss.backward()
             got.append(leaf.grad)
         assert torch.equal(*got) and bool((got[0][:, :385] != 0).all())
+
+
+def test_as_many_columns_as_a_row_may_have():
+    """2^31 - 1 equal logits: their sum and every result but the log-probability's last place are exact; what lies
+    2^31 elements in front of the gradient, where column numbers that wrap around would point, stays as it was."""
+    from fast_jtnn_hip import _capi as K
+    from fast_jtnn_hip import token_log_probs
+
+    v = (1 << 31) - 1
+    x = torch.zeros(1, v, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    labels = torch.tensor([v - 1], device="cuda")
+    lp = token_log_probs(x, labels)
+    assert abs(float(lp) + 31 * np.log(2.0)) <= 2.0 ** -20
+    (d,) = torch.autograd.grad(lp.sum(), x)
+    assert float(d[0, v - 1]) == 1 and int((d[0, :v - 1] != -2.0 ** -31).sum()) == 0
+    del d
+    buf = torch.ones(2 << 31, dtype=torch.bfloat16, device="cuda")
+    out = buf[1 << 31:]
+    stats, coef = torch.tensor([0.0, 2.0 ** 31], device="cuda"), torch.ones(1, device="cuda")
+    g = K.Logits(x.data_ptr(), K.BF16, v, 1, v, labels.data_ptr(), 64)
+    K.label_log_probs_bwd(g, None, stats.data_ptr(), coef.data_ptr(), None, out.data_ptr(), v, v)
+    assert int((buf[:1 << 31] != 1).sum()) == 0 and float(out[v]) == 1
+    assert float(out[v - 1]) == 1 and int((out[:v - 1] != -2.0 ** -31).sum()) == 0
