@@ -536,7 +536,8 @@ int jtvae_label_log_probs(const jtvae_logits_t* logits, const int32_t* owner, fl
 /* dx[i, j] = c_i ([j = label_i] - softmax(x_i)_j) in the logits' type, c_i = coef[owner ? owner[i] : i] * upstream
  * (device scalar, or NULL = 1); rows without a label or with c_i = 0 get zeros, whatever they hold.  Columns
  * [n_cols, width) are padding and become zero (n_cols <= width <= ld_dx).  unless_one: dx holds the gradient for
- * upstream = 1 already and stays as it is if *upstream is 1.  scaled (n_scaled > 0): scaled[q] = coef[q] * upstream. */
+ * upstream = 1 already and stays as it is if *upstream is 1.  scaled (n_scaled > 0): scaled[q] = coef[q] * upstream; with
+ * n_rows = 0 that is all that is done.  An upstream of 0 gives zeros whatever the coefficients are. */
 int jtvae_label_log_probs_bwd(const jtvae_logits_t* logits, const int32_t* owner, const float* stats,
                               const float* coef, const float* upstream, int32_t unless_one, void* dx, int64_t ld_dx,
                               int64_t width, float* scaled, int32_t n_scaled, void* stream);

@@ -381,6 +381,10 @@ __global__ __launch_bounds__(RT* R, NV > 8 ? 4 : RT == 64 && NV == 8 ? 6 : 8) vo
   }
 }
 
+// A coefficient times the upstream factor; a factor of zero leaves out whatever the coefficient is (infinities and NaN of
+// rows that do count).
+__device__ __forceinline__ float times_upstream(float coef, float up) { return up == 0.f ? 0.f : coef * up; }
+
 // dx[row, j] = c ([j = label] - exp(x_j - m) / s), c = coef[owner or row] * upstream, from saved statistics.  Rows are
 // cut into tiles of RT lanes x NV vectors; a block of 256 threads owns 256 / RT tiles.  With unless_one the gradient
 // for an upstream factor of one is in place already and nothing is done where the factor is one.
@@ -396,7 +400,7 @@ __global__ __launch_bounds__(JTVAE_BLOCK) void grad_kernel(RowsIn<T> in, const f
   constexpr int E = Vec<T>::E;
   const float up = upstream ? *upstream : 1.f;
   for (long i = (long)blockIdx.x * JTVAE_BLOCK + threadIdx.x; i < n_scaled; i += (long)gridDim.x * JTVAE_BLOCK)
-    scaled[i] = coef[i] * up;
+    scaled[i] = times_upstream(coef[i], up);
   if (unless_one && up == 1.f) return;
   // Last rows first: they are what the pass that formed the statistics has left in the caches.  Where nothing is due
   // mostly, the grid is smaller than the work and a block takes several pieces.
@@ -420,7 +424,7 @@ __global__ __launch_bounds__(JTVAE_BLOCK) void grad_kernel(RowsIn<T> in, const f
         if (first + u * RT < n_vec)
           w[u] = ONCE ? Vec<T>::load_once(x + shape.col(first + u * RT)) : Vec<T>::load(x + shape.col(first + u * RT));
       const float2 st = in.stats[row];
-      k = coef[own] * up;
+      k = times_upstream(coef[own], up);
       if (label >= in.n_cols && k != 0.f) k = NAN;
       m = finite_or_zero(st.x);
       ks = k / st.y;

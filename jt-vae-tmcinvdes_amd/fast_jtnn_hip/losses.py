@@ -394,8 +394,8 @@ class _PreferenceLoss(torch.autograd.Function):
             d = ctx.gradient(x, labels, plan.arg.row_seq, stats, coef, dloss.data_ptr(), K.ptr(dother),
                              plan.n_seq if want_other else 0)
         elif want_other:
-            at = 2 * x.shape[0]
-            torch.mul(ctx.ws.view(torch.float32)[at:at + plan.n_seq], dloss, out=dother)
+            none = K.Logits(None, K.F32, 1, 0, 1, None, 32)  # no rows: the sequences' coefficients alone
+            K.label_log_probs_bwd(none, None, None, coef, dloss.data_ptr(), None, 1, 1, 0, K.ptr(dother), plan.n_seq)
         if want_other and ctx.other_dtype is not torch.float32:
             dother = dother.to(ctx.other_dtype)
         return d, dother, None, None, None, None, None, None, None, None

@@ -57,3 +57,50 @@ def test_as_many_columns_as_a_row_may_have():
     K.label_log_probs_bwd(g, None, stats.data_ptr(), coef.data_ptr(), None, out.data_ptr(), v, v)
     assert int((buf[:1 << 31] != 1).sum()) == 0 and float(out[v]) == 1
     assert float(out[v - 1]) == 1 and int((out[:v - 1] != -2.0 ** -31).sum()) == 0
+
+
+def test_an_upstream_factor_of_zero_over_rows_that_count():
+    """The usual guard of a loss that is not finite: nothing of a NaN, an infinity or a label outside the vocabulary comes
+    through a factor of zero - neither into the logits' gradient nor into the other terms'."""
+    from fast_jtnn_hip import SequencePlan, policy_loss, preference_loss
+
+    x = torch.randn(6, 385, device="cuda")
+    x[2] = float("nan")
+    x[3, 5] = float("inf")
+    labels = torch.arange(6, device="cuda")
+    labels[4] = 1000
+    old = torch.full((6,), -2.0, device="cuda")
+    old[5] = -2000.0  # the ratio overflows
+    zero, ref = torch.zeros((), device="cuda"), torch.zeros(2, device="cuda")
+    x.requires_grad_()
+    loss = policy_loss(x, labels, old, old, ref_log_probs=old, kl_coef=0.1).loss
+    assert not bool(torch.isfinite(loss))
+    guarded = torch.where(torch.isfinite(loss), loss, zero)
+    assert bool((torch.autograd.grad(loss, x, zero, retain_graph=True)[0] == 0).all())
+    assert bool((torch.autograd.grad(guarded, x)[0] == 0).all())
+    plan = SequencePlan([0, 0, 0, 1, 1, 1], 2, "cuda", pairs=[[0, 1]])
+    for dtype in (torch.float32, torch.float64):
+        other = torch.zeros(2, dtype=dtype, device="cuda", requires_grad=True)
+        for logits, leaves in ((x, (x, other)), (x, (x,)), (x.detach(), (other,))):
+            loss = preference_loss(logits, labels, plan, ref, other_log_probs=other).loss
+            assert not bool(torch.isfinite(loss))
+            for d in torch.autograd.grad(loss, leaves, zero):
+                assert bool((d == 0).all())
+
+
+def test_only_the_other_terms_scaled():
+    """Their gradient alone, with a factor: the coefficients times it, as beside the logits' gradient; without sequences."""
+    from fast_jtnn_hip import SequencePlan, preference_loss
+
+    x = torch.randn(40, 385, device="cuda")
+    labels = torch.randint(0, 385, (40,), device="cuda")
+    plan = SequencePlan(np.arange(40) % 8, 8, "cuda", pairs=np.arange(8).reshape(4, 2))
+    other, ref, three = torch.randn(8, device="cuda", requires_grad=True), torch.zeros(8, device="cuda"), torch.tensor(-3.0, device="cuda")
+    alone = torch.autograd.grad(preference_loss(x, labels, plan, ref, other_log_probs=other).loss, other, three)[0]
+    x.requires_grad_()
+    both = torch.autograd.grad(preference_loss(x, labels, plan, ref, other_log_probs=other).loss, (x, other), three)[1]
+    assert torch.equal(alone, both) and bool((alone != 0).all())
+    none = SequencePlan(np.full(40, -1), 0, "cuda", pairs=np.zeros((0, 2), np.int32))
+    other = torch.zeros(0, device="cuda", requires_grad=True)
+    loss = preference_loss(x.detach(), labels, none, other.detach(), other_log_probs=other).loss
+    assert torch.autograd.grad(loss, other)[0].shape == (0,)
