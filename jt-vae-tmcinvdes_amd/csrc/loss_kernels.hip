@@ -842,9 +842,11 @@ int jtvae_preference_loss(const jtvae_logits_t* logits, const jtvae_sequences_t*
                        margins, dmargin, coef);
     return launch_status();
   }
-  hipLaunchKernelGGL(sequence_sums_kernel, dim3(sum_blocks(n_seq)), dim3(JTVAE_BLOCK), 0, s, q, lp64,
-                     in.other, sums64, sums);
-  JT_CHECK(launch_status());
+  if (n_seq) {  // else every row is without a sequence, and a grid would be empty
+    hipLaunchKernelGGL(sequence_sums_kernel, dim3(sum_blocks(n_seq)), dim3(JTVAE_BLOCK), 0, s, q, lp64,
+                       in.other, sums64, sums);
+    JT_CHECK(launch_status());
+  }
   hipLaunchKernelGGL(preference_kernel<false>, dim3(1), dim3(kPairBlock), 0, s, q, in, lp64, sums64, sums, loss,
                      margins, dmargin, coef);
   return launch_status();

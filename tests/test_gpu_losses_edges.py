@@ -104,3 +104,18 @@ def test_only_the_other_terms_scaled():
     other = torch.zeros(0, device="cuda", requires_grad=True)
     loss = preference_loss(x.detach(), labels, none, other.detach(), other_log_probs=other).loss
     assert torch.autograd.grad(loss, other)[0].shape == (0,)
+
+
+@pytest.mark.parametrize("n", [4096, 4097, 70000])
+def test_no_sequences_over_many_rows(n):
+    """Rows of which none belongs to a sequence, on both sides of the rule that gives the sums a launch of their own."""
+    from fast_jtnn_hip import SequencePlan, preference_loss, sequence_log_probs
+
+    x = torch.randn(n, 7, device="cuda", requires_grad=True)
+    labels = torch.zeros(n, dtype=torch.int64, device="cuda")
+    plan = SequencePlan(np.full(n, -1), 0, "cuda", pairs=np.zeros((0, 2), np.int32))
+    r = preference_loss(x, labels, plan, torch.zeros(0, device="cuda"))
+    assert float(r.loss) == 0 and r.log_probs.shape == (0,) and r.margins.shape == (0,)
+    assert bool((torch.autograd.grad(r.loss, x)[0] == 0).all())
+    sums = sequence_log_probs(x, labels, plan)
+    assert sums.shape == (0,) and bool((torch.autograd.grad(sums.sum(), x)[0] == 0).all())
