@@ -37,7 +37,7 @@
 extern "C" {
 #endif
 
-#define JTVAE_ABI_VERSION 20
+#define JTVAE_ABI_VERSION 21
 
 #define JTVAE_E_NULL (-1)     /* required pointer is NULL            */
 #define JTVAE_E_SHAPE (-2)    /* negative / inconsistent sizes       */
@@ -87,6 +87,10 @@ int jtvae_abi_version(void);
  * reference. */
 uint64_t jtvae_nt_launch_count(void);
 const char* jtvae_error_string(int code);
+
+/* *id (host) = number of the capture that the stream takes part in, which no other capture of the process has; 0 if it
+ * is not being captured.  Memory made inside a capture belongs to that graph alone.  No counterpart in the reference. */
+int jtvae_stream_capture_id(void* stream, uint64_t* id);
 
 /* ---- dense contractions on the matrix cores ------------------------------------------- */
 

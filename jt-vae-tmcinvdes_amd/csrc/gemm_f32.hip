@@ -1602,6 +1602,15 @@ int jtvae_gemm_tn_static(const float* X, int32_t ldx, const int32_t* x_rows, con
 
 int jtvae_abi_version(void) { return JTVAE_ABI_VERSION; }
 
+int jtvae_stream_capture_id(void* stream, uint64_t* id) {
+  if (!id) return JTVAE_E_NULL;
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long n = 0;
+  const hipError_t e = hipStreamGetCaptureInfo((hipStream_t)stream, &status, &n);
+  *id = e == hipSuccess && status == hipStreamCaptureStatusActive ? n : 0;
+  return e == hipSuccess ? 0 : (int)e;
+}
+
 int jtvae_set_small_tile_rows(int rows) {
   const int before = small_rows_override;
   small_rows_override = rows < 0 ? -1 : rows;

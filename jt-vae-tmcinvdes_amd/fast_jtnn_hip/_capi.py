@@ -26,7 +26,7 @@ LIB_PATH = os.environ.get("JTVAE_HIP_LIB") or os.path.join(_HERE, "libjtvae_hip.
 
 ACT_NONE, ACT_RELU, ACT_SIGMOID, ACT_TANH = 0, 1, 2, 3
 EPI_PLAIN, EPI_GRU_BLEND, EPI_MUL_ACC = 0, 1, 2
-ABI_VERSION = 20
+ABI_VERSION = 21
 F32, F16, BF16 = 0, 1, 2
 DTYPE_CODE = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 
@@ -272,6 +272,7 @@ SIGNATURES = {
     "jtvae_onehot_linear": (C.c_int, [_vp, _i32, _i32, _vp, _i32, _vp, _vp, _i32, _i32, _vp]),
     "jtvae_onehot_linear_bwd_workspace_bytes": (_sz, [_i32, _i32, _i32]),
     "jtvae_onehot_linear_bwd": (C.c_int, [_vp, _i32, _i32, _vp, _i32, _i32, _vp, _i32, _i32, _vp, _sz, _vp]),
+    "jtvae_stream_capture_id": (C.c_int, [_vp, C.POINTER(C.c_uint64)]),
     "jtvae_label_log_probs": (C.c_int, [C.POINTER(Logits), _vp, _vp, _vp, _vp, _vp]),
     "jtvae_label_log_probs_bwd": (C.c_int, [C.POINTER(Logits), _vp, _vp, _vp, _vp, _i32, _vp, _i64, _i64, _vp, _i32, _vp]),
     "jtvae_sequence_log_probs_workspace_bytes": (_sz, [_i32]),
@@ -348,6 +349,15 @@ def stream_ptr() -> int:
     if _raw_stream is not None:
         return _raw_stream(torch.cuda.current_device())
     return torch.cuda.current_stream().cuda_stream
+
+
+def capture_id():
+    """Number of the graph capture that the current stream takes part in, None outside of captures."""
+    if not torch.cuda.is_current_stream_capturing():
+        return None
+    out = C.c_uint64()
+    check(lib.jtvae_stream_capture_id(stream_ptr(), C.byref(out)), "stream_capture_id")
+    return out.value
 
 
 def ptr(t, offset_elems: int = 0):

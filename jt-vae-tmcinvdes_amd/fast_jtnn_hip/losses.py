@@ -227,16 +227,17 @@ class _Gradient:
     pass on a thread of its own, which has just been woken and takes two to three times as long over the same Python.
     Buffers of up to ``EARLY_BYTES`` are among it (24 x 385, both passes: 112 -> 90 us on one machine); larger ones
     are not held between the passes.  Nothing made early serves where one of the passes is captured into a graph and the
-    other is not: a replay would write a buffer that is no memory of the graph's, or find one that has been changed."""
+    other is not, or into another one: a replay would write a buffer that is no memory of the graph's, or find one that has
+    been changed."""
 
     EARLY_BYTES = 4 << 20
 
-    __slots__ = ("g", "keep", "place", "buffer", "ld", "made", "captured")
+    __slots__ = ("g", "keep", "place", "buffer", "ld", "made", "capture")
 
     def __init__(self, x, labels, g, keep, want, made=False):
         """``made``: the buffer will hold the gradient for an upstream factor of one when the forward pass ends."""
         self.g, self.keep, self.place = g, keep, self._place(x, labels)
-        self.buffer, self.made, self.captured = None, made, torch.cuda.is_current_stream_capturing()
+        self.buffer, self.made, self.capture = None, made, K.capture_id()
         if want and (made or g.n_rows * g.n_cols * x.element_size() <= self.EARLY_BYTES):
             self.buffer, self.ld = _grad_rows(x)
 
@@ -259,7 +260,7 @@ class _Gradient:
 
     def early(self, buffer):
         """A buffer made with the forward pass, if the backward pass that now runs may use it."""
-        return buffer if buffer is not None and self.captured == torch.cuda.is_current_stream_capturing() else None
+        return buffer if buffer is not None and self.capture == K.capture_id() else None
 
     def __call__(self, x, labels, owner, stats, coef, up, scaled=None, n_scaled=0):
         """The gradient from saved statistics and coefficients (addresses), on the device and stream of the forward pass,

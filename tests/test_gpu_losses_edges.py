@@ -119,3 +119,67 @@ def test_no_sequences_over_many_rows(n):
     assert bool((torch.autograd.grad(r.loss, x)[0] == 0).all())
     sums = sequence_log_probs(x, labels, plan)
     assert sums.shape == (0,) and bool((torch.autograd.grad(sums.sum(), x)[0] == 0).all())
+
+
+def test_capture_ids():
+    """One number per capture, on every stream that takes part; none outside, and none on a stream that does not."""
+    from fast_jtnn_hip import _capi as K
+
+    x = torch.zeros(5, device="cuda")
+    a, b, apart = torch.cuda.Stream(), torch.cuda.Stream(), torch.cuda.Stream()
+    seen = []
+    assert K.capture_id() is None
+    for _ in range(3):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=a):
+            x.add_(1)
+            seen.append(K.capture_id())
+            b.wait_stream(a)
+            with torch.cuda.stream(b):
+                assert K.capture_id() == seen[-1]
+                x.add_(1)
+            with torch.cuda.stream(apart):
+                assert K.capture_id() is None
+            a.wait_stream(b)
+            assert K.capture_id() == seen[-1]
+    assert len(set(seen)) == 3 and None not in seen and K.capture_id() is None
+
+
+def test_passes_captured_into_two_graphs():
+    """The forward pass in one graph, the backward pass in another: every replay of the second writes the whole gradient,
+    whatever became of the last replay's; a replay of both follows the logits."""
+    from fast_jtnn_hip import SequencePlan, policy_loss, preference_loss, sequence_log_probs, token_log_probs
+
+    n, v = 24, 385
+    x = torch.randn(n, v, device="cuda", requires_grad=True)
+    labels = torch.randint(0, v, (n,), device="cuda")
+    plan = SequencePlan(np.arange(n) % 4, 4, "cuda", pairs=[[0, 1], [2, 3]])
+    ref, old = torch.zeros(4, device="cuda"), torch.full((n,), -6.0, device="cuda")
+    other = torch.zeros(4, device="cuda", requires_grad=True)
+    calls = [(lambda: token_log_probs(x, labels).sum(), [x]),
+             (lambda: sequence_log_probs(x, labels, plan).sum(), [x]),
+             (lambda: preference_loss(x, labels, plan, ref, other_log_probs=other).loss, [x, other]),
+             (lambda: policy_loss(x, labels, old, old).loss, [x]),
+             (lambda: policy_loss(x, labels, old, old).loss * 3, [x])]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        [torch.autograd.grad(f(), leaves) for f, leaves in calls]
+    torch.cuda.synchronize()
+    first, second = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(first, stream=side):
+        losses = [f() for f, _ in calls]
+    with torch.cuda.graph(second, stream=side):
+        got = [torch.autograd.grad(loss, leaves, retain_graph=True) for loss, (_, leaves) in zip(losses, calls)]
+    for k in range(3):
+        with torch.no_grad():
+            x.copy_(torch.randn(n, v, device="cuda"))
+        want = [torch.autograd.grad(f(), leaves) for f, leaves in calls]
+        first.replay()
+        for again in range(2):
+            second.replay()
+            torch.cuda.synchronize()
+            for i, (a, b) in enumerate(zip(got, want)):
+                for p, q in zip(a, b):
+                    assert torch.equal(p, q), (k, again, i)
+                    p.fill_(float("nan"))

@@ -59,3 +59,23 @@ def test_saved_tensors_left_on_the_host(monkeypatch):
     x, labels = torch.zeros(6, 8), torch.zeros(6, dtype=torch.int64)
     with pytest.raises(RuntimeError, match="no CPU path"):
         _gradient(x, labels)(x.clone(), labels, None, 1, 1, None)
+
+
+def test_buffers_made_early_serve_the_same_capture_alone(launches, monkeypatch):
+    """Both passes eager or in one capture: the buffer of the forward pass.  Else one of the backward pass's own, made as
+    a whole (the launch is not told that it stands already)."""
+    x, labels = torch.zeros(6, 8), torch.zeros(6, dtype=torch.int64)
+    for made in (False, True):
+        for there, here, same in ((None, None, True), (3, 3, True), (None, 3, False), (3, None, False), (3, 4, False)):
+            monkeypatch.setattr(K, "capture_id", lambda: there)
+            grad = losses._Gradient(x, labels, *losses._arg(x, labels), True, made=made)
+            early, flags = grad.buffer, []
+            monkeypatch.setattr(K, "label_log_probs_bwd", lambda *a: flags.append(a[8]))
+            monkeypatch.setattr(K, "capture_id", lambda: here)
+            d = grad(x, labels, None, 1, 1, None)
+            assert (d is early) == same and flags == [int(made and same)]
+            assert grad(x, labels, None, 1, 1, None) is not d  # given away once
+
+
+def test_capture_id_refused():
+    assert K.lib.jtvae_stream_capture_id(None, None) == K.E_NULL
