@@ -12,7 +12,7 @@ preferred, learning from rewards of sampled ones - needs the log-probability of 
 Logits are [N, V] in fp32, fp16 or bf16, rows at any stride; labels are [N] int32 or int64, a negative label leaves its
 row out (log-probability 0, gradient 0, its logits are never read).  A label >= V gives NaN.  Where the upstream gradient
 or a weight is zero the gradient is zero, whatever the row holds.  Gradients come back in the logits' type and layout, and
-are differentiable once.  Statistics are fp32, sums over a sequence fp64; no atomics, so
+are differentiable once, in reverse mode only.  Statistics are fp32, sums over a sequence fp64; no atomics, so
 results repeat bit for bit.  Every call only enqueues work on the current stream and may be captured; a captured plan
 lives as long as the graph.
 """
@@ -24,6 +24,7 @@ from typing import NamedTuple, Optional
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _capi as K
@@ -130,6 +131,9 @@ def _check(what, logits, labels):
         raise ValueError("%s: %s labels for %d rows" % (what, tuple(labels.shape), logits.shape[0]))
     if labels.dtype not in (torch.int32, torch.int64):
         raise TypeError("%s: int32 or int64 labels are expected, got %s" % (what, labels.dtype))
+    # scoring enters no autograd function, which would refuse it; asking without a level costs 0.6 us
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(logits).tangent is not None:
+        raise NotImplementedError("%s: there is no forward-mode derivative" % what)
     if logits.shape[0] >= 2 ** 31 or logits.shape[1] >= 2 ** 31:
         raise ValueError("%s: logits %s exceed 32-bit row or column numbers" % (what, tuple(logits.shape)))
 

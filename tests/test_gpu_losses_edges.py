@@ -183,3 +183,20 @@ def test_passes_captured_into_two_graphs():
                 for p, q in zip(a, b):
                     assert torch.equal(p, q), (k, again, i)
                     p.fill_(float("nan"))
+
+
+def test_forward_mode_is_refused_with_a_plan_too():
+    """Scoring without reverse mode, plan and logits on the GPU; a level alone changes nothing."""
+    from torch.autograd import forward_ad
+
+    from fast_jtnn_hip import SequencePlan, sequence_log_probs, token_log_probs
+
+    x, labels = torch.randn(4, 7, device="cuda"), torch.zeros(4, dtype=torch.int64, device="cuda")
+    plan = SequencePlan([0, 0, 1, 1], 2, "cuda")
+    calls = [lambda t: token_log_probs(t, labels), lambda t: sequence_log_probs(t, labels, plan)]
+    want = [f(x) for f in calls]
+    with forward_ad.dual_level():
+        for f, w in zip(calls, want):
+            assert torch.equal(f(x), w)
+            with pytest.raises(NotImplementedError):
+                f(forward_ad.make_dual(x, torch.ones_like(x)))

@@ -1,0 +1,28 @@
+"""CPU: calls of the losses at the edges of what they take (the device check comes last)."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from fast_jtnn_hip import SequencePlan, losses
+
+
+def _plan(n_rows, n_seq):
+    """A plan as the constructor leaves it, without its device tables."""
+    p = SequencePlan.__new__(SequencePlan)
+    p.n_rows, p.n_seq, p.n_pairs, p.device = n_rows, n_seq, 1, torch.device("cpu")
+    return p
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_is_refused(grad):
+    """With and without reverse mode recording: no call returns a value that has lost its tangent."""
+    x, labels, f = torch.zeros(4, 7), torch.zeros(4, dtype=torch.int64), torch.zeros(4)
+    calls = [lambda t: losses.token_log_probs(t, labels), lambda t: losses.sequence_log_probs(t, labels, _plan(4, 2)),
+             lambda t: losses.preference_loss(t, labels, _plan(4, 2), f[:2]), lambda t: losses.policy_loss(t, labels, f, f)]
+    with torch.set_grad_enabled(grad), forward_ad.dual_level():
+        for leaf in (x, x.clone().requires_grad_()):
+            for call in calls:
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    call(forward_ad.make_dual(leaf, torch.ones_like(x)))
+                with pytest.raises(RuntimeError, match="no CPU path"):
+                    call(leaf)  # no tangent of its own
