@@ -235,7 +235,7 @@ __device__ __forceinline__ float root(float v) {
 
 struct Step {
   unsigned dice;  // of the tensor and its step; 0: round to nearest
-  float keep, rate, eps, beta1, one_m_beta1, beta2, one_m_beta2, grad_scale, bias2;
+  float decay, rate, eps, beta1, one_m_beta1, beta2, one_m_beta2, grad_scale, bias2;
 };
 
 // The four elements of a tensor from `at`.  8-bit states: a wave's 256 elements are a block, which shares a scale; its
@@ -269,8 +269,10 @@ __device__ __forceinline__ void update(const jtvae_adamw_tensor_t& t, const T* g
     m[k] = fmaf(s.one_m_beta1, x, s.beta1 * m[k]);
     v[k] = s.beta2 * v[k] + s.one_m_beta2 * (x * x);
     r[k] = root(v[k]);
-    // reciprocal on the hardware unit (1 ulp): the update is off by 2^-22 of itself, below half an ulp of w
-    w[k] = w[k] * s.keep - s.rate * (m[k] * __builtin_amdgcn_rcpf(r[k] * s.bias2 + s.eps));
+    // decay and update are one change, rounded into w once: a factor 1 - lr * decay would hold the decay in steps of
+    // 2^-24 (none at all below 2^-25).  Reciprocal on the hardware unit (1 ulp): the update is off by 2^-22 of itself,
+    // which is below half an ulp of weights above eight times their update and shows in smaller ones
+    w[k] -= fmaf(s.rate, m[k] * __builtin_amdgcn_rcpf(r[k] * s.bias2 + s.eps), s.decay * w[k]);
     // a 16-bit parameter is the 32-bit value rounded: the compiler must not round the sum to 16 bits by itself
     if constexpr (sizeof(T) == 2) asm("" : "+v"(w[k]));
   }
@@ -327,7 +329,7 @@ __global__ __launch_bounds__(kBlock) void adamw_kernel(const jtvae_adamw_tensor_
   const float lr = h.lr_device ? *h.lr_device : h.lr;
   // the same rounding for the same step of the same tensor, whatever the launch
   const unsigned dice = BITS == 8 && h.steps ? mix((unsigned)h.steps[c.x] * 0x9e3779b9u + (unsigned)c.x) | 1u : 0u;
-  const Step s = {dice, 1.f - lr * h.decay, lr * b.x,      h.eps, h.beta1, h.one_m_beta1, h.beta2, h.one_m_beta2,
+  const Step s = {dice, lr * h.decay, lr * b.x, h.eps, h.beta1, h.one_m_beta1, h.beta2, h.one_m_beta2,
                   h.grad_scale ? *h.grad_scale : 1.f, b.y};
   if (base + kRound <= t.n) update<T, MASTER, BITS, true>(t, g, s, at);
   else update<T, MASTER, BITS, false>(t, g, s, at);
