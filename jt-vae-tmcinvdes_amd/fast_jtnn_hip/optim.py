@@ -272,12 +272,21 @@ class AdamW(torch.optim.Optimizer):
             torch.autograd.graph.increment_version(changed)
         return loss
 
-    @torch.no_grad()
     def load_state_dict(self, state_dict):
         """Takes the states of a dict of the same parameter groups (this class's, or with ``state_bits=32`` that of
         ``torch.optim.AdamW`` / ``Adam`` without the variants that this class does not step by) into the buffers;
         hyperparameters follow the dict, ``state_bits`` and ``master`` do not.  A learning rate on the device takes its
-        new value in its place.  A parameter without an entry starts afresh."""
+        new value in its place.  A parameter without an entry starts afresh.  Registered hooks run around it."""
+        state_dict = dict(state_dict)  # a hook may change it, not the caller's
+        for hook in self._optimizer_load_state_dict_pre_hooks.values():
+            new = hook(self, state_dict)
+            state_dict = state_dict if new is None else new
+        with torch.no_grad():
+            self._load(state_dict)
+        for hook in self._optimizer_load_state_dict_post_hooks.values():
+            hook(self)
+
+    def _load(self, state_dict):
         groups = state_dict["param_groups"]
         if len(groups) != len(self.param_groups):
             raise ValueError("AdamW: the state dict has %d parameter groups, the optimizer %d"

@@ -30,3 +30,37 @@ def test_small_decay_adds_up(decay, bits, dtype):
         w = w - lr * decay * w - lr * x / (x.abs() + 1.0)
     now = (p.detach() if dtype == torch.float32 else opt.state[p]["master"]).double()
     assert abs(float((now - w).mean())) <= 2e-8 + 1000 * (lr * 16 * U + lr * decay * 4 * U)
+
+
+def test_load_state_dict_hooks():
+    """Hooks run around the load, a dict that one returns is the one that is taken, and what one changes is not the
+    caller's; a refused dict runs none of those after it."""
+    from fast_jtnn_hip import AdamW
+
+    p = torch.nn.Parameter(torch.ones(300, device="cuda"))
+    p.grad = torch.ones_like(p)
+    opt = AdamW([p], lr=1e-3)
+    opt.step()
+    saved, seen = opt.state_dict(), []
+
+    def slower(o, d):
+        seen.append(float(d["param_groups"][0]["lr"]))
+        return dict(d, param_groups=[dict(g, lr=5e-4) for g in d["param_groups"]])
+
+    def changes(o, d):
+        seen.append("changes")
+        d["note"] = 1
+
+    handles = [opt.register_load_state_dict_pre_hook(changes), opt.register_load_state_dict_pre_hook(slower),
+               opt.register_load_state_dict_post_hook(lambda o: seen.append(o.param_groups[0]["lr"]))]
+    opt.load_state_dict(saved)
+    assert seen == ["changes", 1e-3, 5e-4] and "note" not in saved and saved["param_groups"][0]["lr"] == 1e-3
+    del seen[:]
+    handles[1].remove()
+    with pytest.raises(ValueError):
+        opt.load_state_dict({"state": {}, "param_groups": [{"params": [0, 1]}]})
+    assert seen == ["changes"]
+    handles[0].remove()
+    handles[2].remove()
+    opt.load_state_dict(saved)
+    assert seen == ["changes"] and int(opt.state[p]["step"]) == 1
