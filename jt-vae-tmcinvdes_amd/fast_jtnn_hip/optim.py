@@ -69,6 +69,7 @@ class _Group:
         self.addresses = None
         self.table = zeros(C.sizeof(K.AdamwTensor) * len(params), torch.uint8)
         self.grads = (C.c_void_p * len(params))()
+        self.grads_at = C.addressof(self.grads)
         self.views = [self._views(i) for i in range(len(params))]
         if self.master:
             self.copy_master()
@@ -92,7 +93,8 @@ class _Group:
     def bind(self):
         """The device table of addresses; written again, in its place, only when a parameter's storage has moved."""
         addresses = list(map(torch.Tensor.data_ptr, self.params))
-        if addresses == self.addresses:
+        # a parameter may have been turned in its place (p.data = p.data.t()): the elements' order is part of the table
+        if addresses == self.addresses and all(map(torch.Tensor.is_contiguous, self.params)):
             return
         for p, n in zip(self.params, self.numels):
             if p.device != self.device or p.dtype != self.dtype or p.numel() != n or not p.is_contiguous():
@@ -141,7 +143,7 @@ class _Group:
                 lr = float(lr)
         b1, b2 = hyper["betas"]
         return K.AdamwGroup(self.table.data_ptr(), self.chunks.data_ptr(), self.chunk_ptr.ctypes.data,
-                            C.cast(self.grads, C.c_void_p), self.steps.data_ptr(), self.bias.data_ptr(),
+                            self.grads_at, self.steps.data_ptr(), self.bias.data_ptr(),
                             len(self.params), self.n_chunks, K.DTYPE_CODE[self.dtype], self.bits, int(self.master),
                             int(hyper["rounding"] == "stochastic"), lr_dev, lr, b1, b2, hyper["eps"], hyper["weight_decay"])
 

@@ -64,3 +64,30 @@ def test_load_state_dict_hooks():
     handles[2].remove()
     opt.load_state_dict(saved)
     assert seen == ["changes"] and int(opt.state[p]["step"]) == 1
+
+
+def test_a_parameter_turned_in_its_place_is_refused():
+    """Transposed data keep address, size and type, and the old gradient keeps its order; turned back, steps go on."""
+    from fast_jtnn_hip import AdamW
+
+    p, q = (torch.nn.Parameter(torch.randn(40, 40, device="cuda")) for _ in range(2))
+    for t in (p, q):
+        t.grad = torch.randn(40, 40, device="cuda")
+    opt = AdamW([p, q])
+    opt.step()
+    q.data = q.data.t()
+    before = [t.detach().clone() for t in (p, q)]
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="layout"):
+            opt.step()
+    assert all(torch.equal(t, b) for t, b in zip((p, q), before))
+    q.data = q.data.t()
+    opt.step()
+    assert int(opt.state[q]["step"]) == 2 and not torch.equal(p, before[0])
+    one = torch.nn.Parameter(torch.ones(1, 30, device="cuda"))  # a row turned into a column keeps its order
+    opt = AdamW([one], lr=0.25, weight_decay=0.0)
+    for shape in ((1, 30), (30, 1)):
+        one.data = one.data.t() if one.shape != shape else one.data
+        one.grad = torch.ones_like(one)
+        opt.step()
+    assert bool(((one.detach() - 0.5).abs() < 1e-6).all())
