@@ -81,18 +81,30 @@ __device__ __forceinline__ void store(T* p, long i, long n, const float v[N]) {
   }
 }
 
+// Sum of a lane's squares in a chunk: 32 bits over the elements of a load, 64 beyond.  Where one of those overflows, or is so
+// small that squares may have vanished beside it (below 2^-126), all is formed in 64 bits, once more from the registers.
 template <bool WHOLE, typename T>
 __device__ __forceinline__ double chunk_squares(const T* g, long base, long n) {
-  constexpr int N = 16 / sizeof(T);
+  constexpr int N = 16 / sizeof(T), U = JTVAE_ADAMW_CHUNK / (kBlock * N);
+  float v[U][N];
+#pragma unroll
+  for (int u = 0; u < U; ++u) load<WHOLE, false, N>(g, base + (u * kBlock + threadIdx.x) * N, n, v[u]);
   double acc = 0.0;
+  bool fine = true;
 #pragma unroll
-  for (int u = 0; u < JTVAE_ADAMW_CHUNK / (kBlock * N); ++u) {
-    float v[N], s = 0.f;
-    load<WHOLE, false, N>(g, base + (u * kBlock + threadIdx.x) * N, n, v);
+  for (int u = 0; u < U; ++u) {
+    float s = 0.f;
 #pragma unroll
-    for (int k = 0; k < N; ++k) s = fmaf(v[k], v[k], s);
+    for (int k = 0; k < N; ++k) s = fmaf(v[u][k], v[u][k], s);
+    fine = fine && s > 0x1p-80f && s < INFINITY;
     acc += (double)s;
   }
+  if (fine) return acc;
+  acc = 0.0;
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int k = 0; k < N; ++k) acc = fma((double)v[u][k], (double)v[u][k], acc);
   return acc;
 }
 

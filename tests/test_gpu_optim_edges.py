@@ -91,3 +91,41 @@ def test_a_parameter_turned_in_its_place_is_refused():
         one.grad = torch.ones_like(one)
         opt.step()
     assert bool(((one.detach() - 0.5).abs() < 1e-6).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("size", [1e-42, 1e-36, 1e-28, 1e-20, 1e-13, 1.0, 1e15, 1e25, 1e37])
+def test_norms_of_very_small_and_very_large_gradients(size, dtype):
+    """Their squares vanish or overflow in 32 bits, the norm does not; a few ordinary ones among them, and zeros.  Large ones
+    are clipped by it, not brought to nothing: with beta1 = beta2 = 0 and the clipped gradient c far above eps the update is
+    lr c / (|c| + eps), the learning rate but for eps / |c|."""
+    from fast_jtnn_hip import AdamW
+
+    ps = [torch.nn.Parameter(torch.ones(n, device="cuda", dtype=dtype)) for n in (5000, 3, 4097)]
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    for p in ps:
+        p.grad = (torch.randn(p.numel(), generator=gen, device="cuda") * size).to(dtype)
+        p.grad[1::7] = 0
+    want = float(torch.cat([p.grad.double() for p in ps]).square().sum().sqrt())
+    before = [p.detach().clone() for p in ps]
+    opt = AdamW(ps, lr=0.25, betas=(0.0, 0.0), eps=1e-12, weight_decay=0.0, max_norm=1.0)
+    opt.step()
+    if want > torch.finfo(torch.float32).max:  # 1e37 sqrt(7800) = 9e38: no 32-bit number, while the factor is one
+        assert float(opt.grad_norm) == float("inf")
+    else:
+        assert abs(float(opt.grad_norm) - want) <= want * 8 * U + 2.0 ** -149
+    if size >= 1.0:
+        for p, b in zip(ps, before):
+            c = p.grad.double() / want
+            sure = c.abs() > 1e-6  # eps moves these by at most 1e-6 of the update; bf16 parameters follow a 32-bit copy
+            assert bool((((b - p.detach()).double() - 0.25 * c.sign()).abs()[sure] <= 1e-6 + torch.finfo(dtype).eps / 2).all())
+    mixed = torch.nn.Parameter(torch.ones(4096, device="cuda", dtype=dtype))
+    mixed.grad = torch.full_like(mixed, size)
+    mixed.grad[::5] = 1.0
+    opt = AdamW([mixed], max_norm=1.0)
+    opt.step()
+    want = float(mixed.grad.double().square().sum().sqrt())
+    if want > torch.finfo(torch.float32).max:  # 1e37 * 57
+        assert float(opt.grad_norm) == float("inf")
+    else:
+        assert abs(float(opt.grad_norm) - want) <= want * 8 * U
