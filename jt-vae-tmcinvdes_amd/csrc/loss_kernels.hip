@@ -164,7 +164,7 @@ __device__ __forceinline__ PolicyRow policy_row(const PolicyIn& in, int row, dou
   double k3 = 0.0, dk3 = 0.0;
   if (in.ref) {
     const double gap = (double)in.ref[row] - lp, e = expm1(gap);
-    k3 = e - gap;
+    k3 = gap < INFINITY ? e - gap : gap;  // an impossible label's estimate is infinite, not inf - inf
     dk3 = -e;
   }
   const bool penalty = in.kl_coef > 0.0;  // without one an infinite k3 is reported, not multiplied

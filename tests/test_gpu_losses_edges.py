@@ -200,3 +200,24 @@ def test_forward_mode_is_refused_with_a_plan_too():
             assert torch.equal(f(x), w)
             with pytest.raises(NotImplementedError):
                 f(forward_ad.make_dual(x, torch.ones_like(x)))
+
+
+@pytest.mark.parametrize("v", [9, 4099, 70001])
+def test_the_estimate_of_an_impossible_label(v):
+    """A label whose logit is -inf (log-probability -inf) that the reference model gives a chance: an infinite estimate and
+    an infinite loss with a penalty, the loss of its ratio (zero) without one; the other rows' estimates stay."""
+    from fast_jtnn_hip import policy_loss
+
+    inf = float("inf")
+    x = torch.randn(4, v, device="cuda")
+    x[1, 2] = -inf
+    labels, f = torch.full((4,), 2, device="cuda"), torch.full((4,), -8.0, device="cuda")
+    a = torch.tensor([-1.0, 1.0, 1.0, -2.0], device="cuda")
+    out, rest = (policy_loss(t, y, q, b, ref_log_probs=q, clip=(1.0, 1e9)) for t, y, q, b in (
+        (x, labels, f, a), (x[[0, 2, 3]], labels[:3], f[:3], a[[0, 2, 3]])))
+    assert float(out.kl) == inf and float(out.log_probs[1]) == -inf
+    assert abs(float(out.loss) - float(rest.loss)) <= 2.0 ** -22 * abs(float(rest.loss))
+    assert float(policy_loss(x, labels, f, a, ref_log_probs=f, kl_coef=0.1, clip=(1.0, 1e9)).loss) == inf
+    keep = torch.tensor([1.0, 0.0, 1.0, 1.0], device="cuda")
+    out = policy_loss(x, labels, f, a, ref_log_probs=f, weights=keep, kl_coef=0.1)
+    assert bool(torch.isfinite(out.kl)) and bool(torch.isfinite(out.loss))
