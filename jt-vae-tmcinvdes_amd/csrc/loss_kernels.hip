@@ -500,9 +500,10 @@ struct Preference {
 };
 
 // Pairs (a, b): D = beta ((S_a - ref_a) - (S_b - ref_b)), loss = scale sum -(1-e) log sig(D) - e log sig(-D), with
-// -log sig(D) = max(-D, 0) + log1p(exp(-|D|)).  Then the coefficient of every sequence, summed over the pairs that
-// name it in the order of pair_list (pair * 2 + side).  One block, since the loss is one number; with SUMS it also forms
-// the sequences' sums, 16 at a time.
+// -log sig(D) = max(-D, 0) + log1p(exp(-|D|)) and d loss / dD = scale (e sig(D) - (1-e) sig(-D)), both logistic values from
+// exp(-|D|): sig(D) - 1 instead of the second would lose its digits from margins of 20 on.  Then the coefficient of every
+// sequence, summed over the pairs that name it in the order of pair_list (pair * 2 + side).  One block, since the loss is
+// one number; with SUMS it also forms the sequences' sums, 16 at a time.
 template <bool SUMS>
 __global__ __launch_bounds__(kPairBlock) void preference_kernel(Sequences q, Preference in,
                                                                 const double* __restrict__ lp64, double* sums64,
@@ -526,12 +527,12 @@ __global__ __launch_bounds__(kPairBlock) void preference_kernel(Sequences q, Pre
     const int2 ab = q.pairs[p];
     const double d =
         in.beta * ((sums64[ab.x] - (double)in.ref[ab.x]) - (sums64[ab.y] - (double)in.ref[ab.y]));
-    const double l = log1p(exp(-fabs(d)));
+    const double t = exp(-fabs(d)), l = log1p(t), far = t / (1.0 + t), near = 1.0 / (1.0 + t);
     if (in.smoothing < 1.0) acc += (1.0 - in.smoothing) * (fmax(-d, 0.0) + l);  // no 0 * inf at an infinite margin
     if (in.smoothing > 0.0) acc += in.smoothing * (fmax(d, 0.0) + l);
     if (d != d) acc = d;  // fmax drops a NaN
     margins[p] = (float)d;
-    dmargin[p] = in.scale * in.beta * (1.0 / (1.0 + exp(-d)) - (1.0 - in.smoothing));
+    dmargin[p] = in.scale * in.beta * (in.smoothing * (d < 0.0 ? far : near) - (1.0 - in.smoothing) * (d < 0.0 ? near : far));
   }
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) acc += __shfl_xor(acc, off, 64);

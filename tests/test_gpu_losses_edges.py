@@ -221,3 +221,25 @@ def test_the_estimate_of_an_impossible_label(v):
     keep = torch.tensor([1.0, 0.0, 1.0, 1.0], device="cuda")
     out = policy_loss(x, labels, f, a, ref_log_probs=f, weights=keep, kl_coef=0.1)
     assert bool(torch.isfinite(out.kl)) and bool(torch.isfinite(out.loss))
+
+
+@pytest.mark.parametrize("smoothing", [0.0, 0.125, 1.0])
+def test_coefficients_of_far_margins(smoothing):
+    """Against the derivative in 64 bits, relative to itself: two logistic values, each good to a few 2^-53, and one rounding
+    to 32 bits (2^-24, and 2^-149 where the result leaves the normal range)."""
+    from fast_jtnn_hip import SequencePlan, preference_loss
+
+    margins = torch.tensor([-90.0, -60.0, -37.0, -25.0, -15.0, -1.0, 0.0, 0.5, 10.0, 20.0, 30.0, 37.0, 45.0, 90.0], device="cuda")
+    p = len(margins)
+    pairs = np.arange(2 * p).reshape(p, 2)
+    x = torch.zeros(2 * p, 3, device="cuda")
+    other = torch.zeros(2 * p, device="cuda", requires_grad=True)
+    ref = torch.zeros(2 * p, device="cuda")
+    ref[1::2] = margins
+    r = preference_loss(x, torch.zeros(2 * p, dtype=torch.int64, device="cuda"), SequencePlan(np.arange(2 * p), 2 * p, "cuda",
+                        pairs=pairs), ref, beta=1.0, label_smoothing=smoothing, other_log_probs=other, scale=1.0)
+    (d,) = torch.autograd.grad(r.loss, other)
+    m = margins.double()
+    want = smoothing / (1 + torch.exp(-m)) - (1 - smoothing) / (1 + torch.exp(m))
+    assert torch.equal(r.margins, margins)
+    assert bool(((d[::2].double() - want).abs() <= want.abs() * 2.0 ** -23 + 2.0 ** -149).all()) and torch.equal(d[::2], -d[1::2])
