@@ -64,6 +64,8 @@ class SequencePlan:
 
     def __init__(self, row_seq, n_seq, device, pairs=None):
         row_seq = np.ascontiguousarray(_host(row_seq))
+        if row_seq.shape == (0,):  # an empty list has no type of its own
+            row_seq = row_seq.astype(np.int32)
         if row_seq.ndim != 1 or row_seq.dtype.kind not in "iu":
             raise ValueError("row_seq: a list of integers is expected, got %s %s" % (row_seq.dtype, row_seq.shape))
         n_seq = int(n_seq)

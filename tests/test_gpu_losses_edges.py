@@ -243,3 +243,11 @@ def test_coefficients_of_far_margins(smoothing):
     want = smoothing / (1 + torch.exp(-m)) - (1 - smoothing) / (1 + torch.exp(m))
     assert torch.equal(r.margins, margins)
     assert bool(((d[::2].double() - want).abs() <= want.abs() * 2.0 ** -23 + 2.0 ** -149).all()) and torch.equal(d[::2], -d[1::2])
+
+
+def test_a_plan_of_an_empty_list():
+    from fast_jtnn_hip import SequencePlan, sequence_log_probs
+
+    x, labels = torch.zeros(0, 5, device="cuda"), torch.zeros(0, dtype=torch.int64, device="cuda")
+    assert torch.equal(sequence_log_probs(x, labels, SequencePlan([], 3, "cuda")), torch.zeros(3, device="cuda"))
+    assert sequence_log_probs(x, labels, SequencePlan([], 0, "cuda", pairs=[])).shape == (0,)

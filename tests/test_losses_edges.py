@@ -26,3 +26,13 @@ def test_forward_mode_is_refused(grad):
                     call(forward_ad.make_dual(leaf, torch.ones_like(x)))
                 with pytest.raises(RuntimeError, match="no CPU path"):
                     call(leaf)  # no tangent of its own
+
+
+def test_a_plan_of_an_empty_list():
+    """Nothing to refuse but the device: a batch may have no rows."""
+    for rows, pairs in (([], None), ([], []), ((), [[0, 1]])):
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            SequencePlan(rows, 2, "cpu", pairs=pairs)
+    for rows in ([[]], [["a"]]):
+        with pytest.raises(ValueError, match="row_seq"):
+            SequencePlan(rows, 2, "cpu")
