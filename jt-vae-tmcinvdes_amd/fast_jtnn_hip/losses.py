@@ -63,12 +63,13 @@ class SequencePlan:
     other) sequence of every pair; a sequence may appear in several pairs."""
 
     def __init__(self, row_seq, n_seq, device, pairs=None):
-        row_seq = np.ascontiguousarray(_host(row_seq))
+        row_seq, n_seq = _numbers("rows", _host(row_seq), 1), int(n_seq)
+        if n_seq >= 2 ** 31 - 1:
+            raise ValueError("%d sequences exceed 32-bit numbers" % n_seq)
         if row_seq.shape == (0,):  # an empty list has no type of its own
             row_seq = row_seq.astype(np.int32)
         if row_seq.ndim != 1 or row_seq.dtype.kind not in "iu":
             raise ValueError("row_seq: a list of integers is expected, got %s %s" % (row_seq.dtype, row_seq.shape))
-        n_seq = int(n_seq)
         if n_seq < 0:
             raise ValueError("n_seq is %d" % n_seq)
         if row_seq.size and (int(row_seq.min()) < -1 or int(row_seq.max()) >= n_seq):
@@ -79,7 +80,7 @@ class SequencePlan:
         keyptr, order = K.prep_group_by_key(np.where(row_seq < 0, n_seq, row_seq), n_seq + 1)
         self.n_pairs = None
         if pairs is not None:
-            pairs = np.ascontiguousarray(_host(pairs))
+            pairs = _numbers("pairs", _host(pairs), 2)  # every pair has two entries in the tables
             if pairs.size == 0:
                 pairs = np.zeros((0, 2), dtype=np.int32)
             if pairs.ndim != 2 or pairs.shape[1] != 2 or pairs.dtype.kind not in "iu":
@@ -119,6 +120,13 @@ class SequencePlan:
 
 def _host(a):
     return a.detach().cpu().numpy() if isinstance(a, torch.Tensor) else np.asarray(a)
+
+
+def _numbers(what, a, per):
+    """A host array whose entries, ``per`` of a kind, have 32-bit numbers."""
+    if a.ndim and a.shape[0] * per >= 2 ** 31:
+        raise ValueError("%d %s exceed 32-bit numbers" % (a.shape[0], what))
+    return np.ascontiguousarray(a)
 
 
 def _check(what, logits, labels):

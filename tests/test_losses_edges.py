@@ -1,4 +1,5 @@
 """CPU: calls of the losses at the edges of what they take (the device check comes last)."""
+import numpy as np
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -36,3 +37,14 @@ def test_a_plan_of_an_empty_list():
     for rows in ([[]], [["a"]]):
         with pytest.raises(ValueError, match="row_seq"):
             SequencePlan(rows, 2, "cpu")
+
+
+def test_plans_beyond_32_bit_numbers_refused():
+    """Before anything of that size is made (the arrays here are one number, repeated)."""
+    zero = np.zeros((), np.int32)
+    for rows, n_seq, pairs in (([0], 2 ** 31 - 1, None), ([0], 2 ** 32 + 1, None), (np.broadcast_to(zero, (2 ** 31,)), 1, None),
+                               ([0], 1, np.broadcast_to(zero, (2 ** 30, 2)))):
+        with pytest.raises(ValueError, match="32-bit"):
+            SequencePlan(rows, n_seq, "cpu", pairs=pairs)
+    with pytest.raises(ValueError, match="n_seq is"):
+        SequencePlan([0], -2 ** 33, "cpu")
