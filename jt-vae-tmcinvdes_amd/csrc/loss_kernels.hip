@@ -24,6 +24,10 @@ inline int launch_status() {
 
 inline unsigned grid_for(long total) { return (unsigned)((total + JTVAE_BLOCK - 1) / JTVAE_BLOCK); }
 
+// exp(x) on the hardware's exp2.  The product with log2 e is rounded, so the result is off by up to |x| 2^-24 relative to
+// itself: far from the maximum, where a softmax is small, as much as the difference x - max is rounded by anyway.  Making up
+// for what the product loses brings the worst element of fp32 gradients (standard deviation 4) from 2^-18.5 to 2^-19.6 of itself
+// and the log-probabilities nowhere (1e-6 at 780 columns both ways), for 13.6 -> 15.7 us of statistics at 20480 x 780.
 __device__ __forceinline__ float exp_nat(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 
 struct Labels {

@@ -238,7 +238,8 @@ __device__ __forceinline__ unsigned quantise(const float v[4], float top, bool b
   return pack_e4m3(x);
 }
 
-// sqrt on the hardware unit (1 ulp), with what it would flush brought into its range first.
+// sqrt on the hardware unit (1 ulp), with what it would flush brought into its range first.  Rounded correctly it takes 4 %
+// of a whole step more (477 M bf16 elements, 8-bit states: 1432 us against 1377).
 __device__ __forceinline__ float root(float v) {
   const bool low = v < 0x1p-96f;
   const float r = __builtin_amdgcn_sqrtf(low ? v * 0x1p96f : v);
@@ -282,8 +283,9 @@ __device__ __forceinline__ void update(const jtvae_adamw_tensor_t& t, const T* g
     v[k] = s.beta2 * v[k] + s.one_m_beta2 * (x * x);
     r[k] = root(v[k]);
     // decay and update are one change, rounded into w once: a factor 1 - lr * decay would hold the decay in steps of
-    // 2^-24 (none at all below 2^-25).  Reciprocal on the hardware unit (1 ulp): the update is off by 2^-22 of itself,
-    // which is below half an ulp of weights above eight times their update and shows in smaller ones
+    // 2^-24 (none at all below 2^-25).  Reciprocal on the hardware unit (1 ulp): first steps from zero, which are the
+    // update itself, are off by up to 5.2 * 2^-24 of themselves (1e5 elements), 4.7 with a correctly rounded quotient, which
+    // takes 0.2 % longer
     w[k] -= fmaf(s.rate, m[k] * __builtin_amdgcn_rcpf(r[k] * s.bias2 + s.eps), s.decay * w[k]);
     // a 16-bit parameter is the 32-bit value rounded: the compiler must not round the sum to 16 bits by itself
     if constexpr (sizeof(T) == 2) asm("" : "+v"(w[k]));

@@ -129,3 +129,20 @@ def test_norms_of_very_small_and_very_large_gradients(size, dtype):
         assert float(opt.grad_norm) == float("inf")
     else:
         assert abs(float(opt.grad_norm) - want) <= want * 8 * U
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_first_steps_of_weights_that_start_at_zero(bits):
+    """Their first step is the update itself.  Relative to it: g 1 / (1 - beta1) by two roundings and the correction's one,
+    the root 2^-23 and half of what its square (three roundings, the correction's one) is off by, the sum with eps by one, the
+    reciprocal by two, the product with it, the learning rate times its correction and the last product by one each: 13 * 2^-24
+    together where all lean one way."""
+    from fast_jtnn_hip import AdamW
+
+    p = torch.nn.Parameter(torch.zeros(100_000, device="cuda"))
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    p.grad = torch.randn(p.numel(), generator=gen, device="cuda") * torch.exp(3 * torch.randn(p.numel(), generator=gen, device="cuda"))
+    AdamW([p], lr=1e-3, eps=1e-3, weight_decay=0.5, state_bits=bits).step()
+    g = p.grad.double()
+    want = -float(np.float32(1e-3)) * g / (g.abs() + float(np.float32(1e-3)))
+    assert float((p.detach().double() / want - 1).abs().max()) <= 13 * U
