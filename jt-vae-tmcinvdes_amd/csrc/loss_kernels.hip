@@ -716,7 +716,8 @@ int row_grad(const jtvae_logits_t* g, const int32_t* owner, const float* stats, 
   const RowsIn<T> in = rows_in<T>(g, owner, (float*)stats, nullptr, nullptr);
   const GradOut<T> out = {(T*)dx, (long)ld_dx, (long)width};
   const int n_vec = g->n_cols / Vec<T>::E;
-  if (n_vec <= 128) return launch_grad<T, 64, 2, false>(in, coef, upstream, unless_one, out, scaled, n_scaled, s);
+  // Up to 256 vectors a wave takes the row (20480 rows of 129: 14.9 us, in tiles of a block 21.1; of 255: 26.6 and 27.6).
+  // Half as many vectors a lane for rows of up to 128 are no faster (96: 11.1 us both ways).
   if (n_vec <= 256) return launch_grad<T, 64, 4, false>(in, coef, upstream, unless_one, out, scaled, n_scaled, s);
   // Logits beyond what the 256 MiB cache keeps are read past it (forward and backward of 4096 x 128000 bf16: 482 us, 493
   // through it); smaller ones are found there (4000 x 3500 bf16 11.0 us, 12.7 past it).
