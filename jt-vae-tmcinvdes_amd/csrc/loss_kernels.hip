@@ -275,7 +275,9 @@ enum { kStats = 0, kPolicy = 1 };
 // row depending on nothing else, its gradient in the same pass.  A block of RT * R threads owns R rows; the 64-bit
 // arithmetic of a row's end is done by one lane per row, side by side.  Bound by memory: 8192 x 32000 bf16 185 us in 512
 // threads x 8 vectors, 5.4 TB/s read and written (256 x 16 the same, 1024 x 4 199); 4096 x 128000 bf16, where a row
-// takes the registers of a CU and loads and stores do not overlap, 428 us, 4.9 TB/s - the two passes take 538.
+// takes the registers of a CU and loads and stores do not overlap, 428 us, 4.9 TB/s - the two passes take 538.  Eight waves
+// a SIMD leave the forms of 256 and 512 lanes 12 to 20 bytes a lane short of registers; six, which spill nothing, take 181
+// us at 8192 x 32000 bf16 but 43.0 instead of 39.5 at 8192 x 5000.
 template <typename T, int RT, int R, int NV, int MODE>
 __global__ __launch_bounds__(RT* R, NV > 8 ? 4 : RT == 64 && NV == 8 ? 6 : 8) void rows_kernel(
     RowsIn<T> in, PolicyIn policy, float* __restrict__ coef, double* __restrict__ terms, long n_terms, GradOut<T> out) {
@@ -673,8 +675,9 @@ int launch_stats(const RowsIn<T>& rows, hipStream_t s) {
   });
 }
 
-// Statistics.  Rows of up to 512 vectors (8 KiB) sit in a wave's registers, eight waves side by side (60000 x 1500 fp32
-// 58 us, 97 when streamed); longer ones are streamed by a block each.  Up to a row per CU the block has 512 threads, since
+// Statistics.  Rows of up to 512 vectors (8 KiB) sit in a wave's registers, eight waves side by side; longer ones are
+// streamed by a block each.  20480 fp32 rows of 129 vectors 11.5 us, streamed 24.0; of 511 30.8 and 36.9; 513, streamed, 39.9.
+// Two vectors a lane do for 128 (rows of 127: 10.8 us, with eight 11.2; policy pass 26.3 and 27.5).  Up to a row per CU the block has 512 threads, since
 // a CU alone is bound by its arithmetic (64 x 128000 bf16 10.7 us against 14.3, 256 rows 12.9 against 15.6); beyond, 256,
 // so that a CU has blocks at every stage (1024 x 30000 12.9 against 13.9, with 1024 threads 16.3).  Bound by memory from
 // there on: 4096 x 128000 bf16 178 us, 5.9 TB/s read.
@@ -842,7 +845,9 @@ int jtvae_preference_loss(const jtvae_logits_t* logits, const jtvae_sequences_t*
                          preference->label_smoothing, preference->scale};
   JT_CHECK(jtvae_label_log_probs(logits, sequences->row_seq, stats, nullptr, lp64, stream));
   // For a few short sequences the one block of the pairs forms their sums as well, and a launch is saved (16 of 20 rows:
-  // 7.6 us instead of 10.1); else a wave each (64 of 300 rows: 15.8 us instead of 25.4, 1024 of 20: 14.8 instead of 66).
+  // 7.3 us instead of 9.8, in a graph 7.0 and 7.9); else a wave each (64 of 130 rows: 11.6 us instead of 16.2).  At the
+  // limits the two are alike: 64 sequences of 20 rows 9.9 and 10.2, of 64 rows 10.8 and 10.2; 16 of 250 9.7 and 10.4, of 1000
+  // 18.7 and 18.0; 128 of 20 13.6 and 10.1.
   if (n_seq <= 64 && n <= 4096) {
     hipLaunchKernelGGL(preference_kernel<true>, dim3(1), dim3(kPairBlock), 0, s, q, in, lp64, sums64, sums, loss,
                        margins, dmargin, coef);

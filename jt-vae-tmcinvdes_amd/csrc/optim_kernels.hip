@@ -207,7 +207,8 @@ __device__ __forceinline__ float block_top(const float v[4]) {
   return t;
 }
 
-// Well mixed bits of a counter (xor-shifts and odd multipliers; every output once over all counters).
+// Well mixed bits of a counter (xor-shifts and odd multipliers; every output once over all counters).  The shifts and
+// multipliers are the ones published by C. Wellons, "Prospecting for Hash Functions" (2018).
 __device__ __forceinline__ unsigned mix(unsigned x) {
   x = (x ^ (x >> 16)) * 0x7feb352du;
   x = (x ^ (x >> 15)) * 0x846ca68bu;

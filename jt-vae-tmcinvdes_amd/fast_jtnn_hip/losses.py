@@ -14,7 +14,8 @@ row out (log-probability 0, gradient 0, its logits are never read).  A label >= 
 or a weight is zero the gradient is zero, whatever the row holds.  Gradients come back in the logits' type and layout, and
 are differentiable once, in reverse mode only.  Statistics are fp32, sums over a sequence fp64; no atomics, so
 results repeat bit for bit.  Every call only enqueues work on the current stream and may be captured; a captured plan
-lives as long as the graph.
+lives as long as the graph.  Making a ``SequencePlan`` is not such a call: its tables are grouped on the host and copied
+with a wait.
 """
 from __future__ import annotations
 
@@ -239,10 +240,11 @@ def _scratch(device, *counts):
 class _Gradient:
     """The gradient of a call's logits.  What can be made ready is made with the forward pass: autograd runs the backward
     pass on a thread of its own, which has just been woken and takes two to three times as long over the same Python.
-    Buffers of up to ``EARLY_BYTES`` are among it (24 x 385, both passes: 112 -> 90 us on one machine); larger ones
-    are not held between the passes.  Nothing made early serves where one of the passes is captured into a graph and the
-    other is not, or into another one: a replay would write a buffer that is no memory of the graph's, or find one that has
-    been changed."""
+    Buffers of up to ``EARLY_BYTES`` are among it (both passes of ``token_log_probs`` 24 x 385: 103 -> 100 us, of
+    ``preference_loss`` 320 x 385: 141 -> 135, an empty autograd function on the same machine: 50); larger ones
+    are not held between the passes.  Nothing made early serves where one of the passes is captured into a graph and the other
+    is not, or into another one: a replay would write a buffer that is no memory of the graph's, or find one that has been
+    changed."""
 
     EARLY_BYTES = 4 << 20
 
@@ -487,7 +489,9 @@ def policy_loss(logits: torch.Tensor, labels: torch.Tensor, old_log_probs: torch
     with a negative label or a weight of zero do not count, whatever their other inputs hold; ``weights`` (default 1) carry
     masks and means.  Differentiable in ``logits``; the
     other inputs are constants.  The gradient is made along with the loss, for a factor of one on it: a factor is best
-    given as ``scale`` (another one in the backward pass is right too, and makes the gradient a second time)."""
+    given as ``scale`` (another one in the backward pass is right too, and makes the gradient a second time).  Until the
+    backward pass the graph holds that gradient, which is as large as the logits and no saved tensor: hooks that offload
+    those, and checkpointing, do not see it."""
     what = "policy_loss"
     _check(what, logits, labels)
     given = dict(old_log_probs=old_log_probs, advantages=advantages, ref_log_probs=ref_log_probs, weights=weights)

@@ -1,8 +1,9 @@
 """AdamW over many tensors at once on the package's kernels, states in 32 or in 8 bits.
 
 ``AdamW`` is a ``torch.optim.Optimizer`` (learning-rate schedulers, parameter groups and state dicts work as usual).  A
-step is one launch per group whatever the number of tensors, two more if the gradients' global 2-norm is clipped
-(``max_norm``), and nothing of it waits on the host.
+step is two launches per group whatever the number of tensors (step counts and bias corrections; the update), one more if
+the gradients' global 2-norm is clipped (``max_norm``), the same again for every further 400 tensors, and nothing of it waits
+on the host.
 
 States live in one buffer per group and kind; ``optimizer.state[p]`` holds views of them.  With ``state_bits=8`` the
 first moment and the square root of the second are kept as e4m3 values with one fp32 scale per 256 elements: 2.03 bytes
@@ -10,8 +11,9 @@ per parameter instead of 8.  Such a value has three bits behind the point, and a
 less than half a place: rounded to nearest, an element's share in its block stands still until a gradient is eight to
 eleven times its root, and only the block's scale follows the gradients.  ``rounding="stochastic"`` rounds to one of the
 two neighbours with the right mean instead (by bits that are a function of element, tensor and step: runs repeat), so
-that every element follows its own gradients, within some 15 % of the root.  16-bit parameters are stepped on an fp32
-copy (``master=True``), since a step is usually smaller than half their last place.
+that every element follows its own gradients, within some 15 % of the root, for 9 % more time where the step is bound by
+memory (477 M bf16 elements: 1362 -> 1488 us; the trainer's 5.1 M: 25 -> 26 on the device).  16-bit parameters are stepped
+on an fp32 copy (``master=True``), since a step is usually smaller than half their last place.
 """
 from __future__ import annotations
 
