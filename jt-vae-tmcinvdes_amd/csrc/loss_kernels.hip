@@ -677,10 +677,11 @@ int launch_stats(const RowsIn<T>& rows, hipStream_t s) {
 
 // Statistics.  Rows of up to 512 vectors (8 KiB) sit in a wave's registers, eight waves side by side; longer ones are
 // streamed by a block each.  20480 fp32 rows of 129 vectors 11.5 us, streamed 24.0; of 511 30.8 and 36.9; 513, streamed, 39.9.
-// Two vectors a lane do for 128 (rows of 127: 10.8 us, with eight 11.2; policy pass 26.3 and 27.5).  Up to a row per CU the block has 512 threads, since
-// a CU alone is bound by its arithmetic (64 x 128000 bf16 10.7 us against 14.3, 256 rows 12.9 against 15.6); beyond, 256,
-// so that a CU has blocks at every stage (1024 x 30000 12.9 against 13.9, with 1024 threads 16.3).  Bound by memory from
-// there on: 4096 x 128000 bf16 178 us, 5.9 TB/s read.
+// Two vectors a lane do for 128 (rows of 127: 10.8 us, with eight 11.2; policy pass 26.3 and 27.5).  Up to a row per CU the
+// block has 512 threads, since a CU alone is bound by its arithmetic (64 x 128000 bf16 10.7 us against 14.3, 256 rows 12.9
+// against 15.6); beyond, 256, so that a CU has blocks at every stage (1024 x 30000 12.9 against 13.9, with 1024 threads
+// 16.3).  Bound by memory from there on: 4096 x 128000 bf16 178 us, 5.9 TB/s read; a launch of 50 us loses 5 of them to its
+// start and drain (4096 x 32000 5.3 TB/s, 16384 x 32000 6.0).
 template <typename T>
 int row_stats(const jtvae_logits_t* g, const int32_t* owner, float* stats, float* lp32, double* lp64, hipStream_t s) {
   const RowsIn<T> in = rows_in<T>(g, owner, stats, lp32, lp64);

@@ -287,7 +287,8 @@ __device__ __forceinline__ void update(const jtvae_adamw_tensor_t& t, const T* g
     // 2^-24 (none at all below 2^-25).  Reciprocal on the hardware unit (1 ulp): first steps from zero, which are the
     // update itself, are off by up to 5.2 * 2^-24 of themselves (1e5 elements), 4.7 with a correctly rounded quotient, which
     // takes 0.2 % longer
-    w[k] -= fmaf(s.rate, m[k] * __builtin_amdgcn_rcpf(r[k] * s.bias2 + s.eps), s.decay * w[k]);
+    const float shrink = fabsf(w[k]) < INFINITY ? s.decay * w[k] : 0.f;  // an infinite weight stays
+    w[k] -= fmaf(s.rate, m[k] * __builtin_amdgcn_rcpf(r[k] * s.bias2 + s.eps), shrink);
     // a 16-bit parameter is the 32-bit value rounded: the compiler must not round the sum to 16 bits by itself
     if constexpr (sizeof(T) == 2) asm("" : "+v"(w[k]));
   }

@@ -146,3 +146,27 @@ def test_first_steps_of_weights_that_start_at_zero(bits):
     g = p.grad.double()
     want = -float(np.float32(1e-3)) * g / (g.abs() + float(np.float32(1e-3)))
     assert float((p.detach().double() / want - 1).abs().max()) <= 13 * U
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype,master", [(torch.float32, True), (torch.bfloat16, True), (torch.float16, False)])
+def test_infinite_weights_stay(dtype, master, bits):
+    """Masks kept among the parameters: an infinite weight is infinite after a step, with and without decay, for zero and
+    other gradients, and leaves its neighbours alone; a weight that is NaN stays NaN."""
+    from fast_jtnn_hip import AdamW
+
+    inf = float("inf")
+    for decay in (0.0, 0.125):
+        p = torch.nn.Parameter(torch.ones(600, device="cuda", dtype=dtype))
+        with torch.no_grad():
+            p[3::10], p[4::10], p[5] = -inf, inf, float("nan")
+        p.grad = torch.zeros_like(p)
+        p.grad[300:] = 0.5
+        opt = AdamW([p], lr=0.25, weight_decay=decay, state_bits=bits, master=master)
+        opt.step()
+        w = p.detach().float()
+        assert bool((w[3::10] == -inf).all()) and bool((w[4::10] == inf).all()) and bool(torch.isnan(w[5]))
+        kept = 1 - 0.25 * decay
+        want = torch.where(torch.arange(600, device="cuda") < 300, kept, kept - 0.25)
+        rest = torch.isfinite(w)
+        assert int(rest.sum()) == 600 - 121 and bool(((w - want).abs()[rest] <= 1e-6 + torch.finfo(dtype).eps / 2).all())
