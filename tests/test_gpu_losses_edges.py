@@ -251,3 +251,25 @@ def test_a_plan_of_an_empty_list():
     x, labels = torch.zeros(0, 5, device="cuda"), torch.zeros(0, dtype=torch.int64, device="cuda")
     assert torch.equal(sequence_log_probs(x, labels, SequencePlan([], 3, "cuda")), torch.zeros(3, device="cuda"))
     assert sequence_log_probs(x, labels, SequencePlan([], 0, "cuda", pairs=[])).shape == (0,)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_differences_of_long_sums(dtype):
+    """Equal logits: a row's sum is its number of columns exactly, so its log-probability is off by the logarithm's 2^-53
+    alone, and a sequence's by one more per addition.  Sums of hundreds of thousands of such rows lie beyond the last place
+    of 32-bit numbers; their differences to references nearby do not: log-probabilities rounded to 32 bits (each off by
+    1e-8 and more, the same way) would show as 1e-3."""
+    from fast_jtnn_hip import SequencePlan, preference_loss
+
+    n, v = 300_000, 3
+    x = torch.full((n, v), 0.5, dtype=dtype, device="cuda")
+    labels = torch.arange(n, device="cuda") % v
+    row_seq = np.where(np.arange(n) % 3 < 2, 0, 1)
+    want = -np.log(3.0) * np.bincount(row_seq).astype(np.float64)
+    ref = torch.tensor([want[0] - 0.375, want[1] + 1.25], device="cuda", dtype=torch.float32)
+    near = want - ref.double().cpu().numpy()
+    r = preference_loss(x, labels, SequencePlan(row_seq, 2, "cuda", pairs=[[0, 1]]), ref, beta=1.0)
+    exact = near[0] - near[1]
+    off = n * abs(want).max() * 2.0 ** -52  # 1.5e-5
+    assert abs(float(r.margins[0]) - exact) <= abs(exact) * 2.0 ** -24 + off
+    assert abs(float(r.loss) - np.log1p(np.exp(-exact))) <= 2.0 ** -22 + off
