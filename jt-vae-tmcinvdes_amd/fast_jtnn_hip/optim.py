@@ -70,7 +70,7 @@ class _Group:
         self.partials = zeros(max(self.n_chunks, 1), torch.float64)
         self.addresses = None
         self.table = zeros(C.sizeof(K.AdamwTensor) * len(params), torch.uint8)
-        self.grads = (C.c_void_p * len(params))()
+        self.grads, self.grad_list = (C.c_void_p * len(params))(), None
         self.grads_at = C.addressof(self.grads)
         self.views = [self._views(i) for i in range(len(params))]
         if self.master:
@@ -116,6 +116,11 @@ class _Group:
         self.table.copy_(torch.from_numpy(host))
         self.addresses = addresses
 
+    def _name_grads(self, addresses):
+        """The address list of the launches, written where it changed (gradients mostly stay where they are)."""
+        if addresses != self.grad_list:
+            self.grads[:] = self.grad_list = addresses
+
     def gather_grads(self):
         """Fills the address list; (parameters with a gradient, tensors to keep alive until the launches)."""
         grads, dt, T = list(map(_GRAD, self.params)), self.dtype, torch.Tensor
@@ -125,12 +130,12 @@ class _Group:
         except TypeError:  # None among them
             plain = False
         if plain:
-            self.grads[:] = list(map(T.data_ptr, grads))
+            self._name_grads(list(map(T.data_ptr, grads)))
             return self.params, grads
         if any(g is not None and g.numel() != n for g, n in zip(grads, self.numels)):
             raise RuntimeError("AdamW: a gradient has another size than its parameter had when the optimizer was built")
         grads = [None if g is None else g.detach().to(dt).contiguous() for g in grads]
-        self.grads[:] = [None if g is None else g.data_ptr() for g in grads]
+        self._name_grads([None if g is None else g.data_ptr() for g in grads])
         return [p for p, g in zip(self.params, grads) if g is not None], grads
 
     def args(self, hyper):
